@@ -142,6 +142,66 @@ int tbv_step_noalloc(void* out, const void* local, const void* received, void* b
                      size_t nbytes, int dtype, unsigned long long* pack_word, unsigned long long* done_word,
                      unsigned long long seq, void* stream);
 
+/* ------------------------------------------------------------------ Part 3: the layer around the all-reduce
+ *
+ * The operators between two all-reduces of a tensor-parallel decoder layer with int8 weights: rows to int8 codes, the
+ * scaled int8 product (whose row-parallel form gives the all-reduce its operand), rotary positions of the heads.  They have
+ * no counterpart in the reference.  Like tbv_step_noalloc they work on the caller's buffers only: no tbv_ar_init, no
+ * allocation, no workspace, no state between calls; any thread, any stream, stream capture included (the device of
+ * `stream` must be current).  Return 0; -1 after a "[tbvcoll] ..." line on stderr for bad arguments or a launch failure.
+ * Strides are in elements; the last dimension is contiguous. */
+
+/* Rows of `hidden` elements of `dtype` to int8 codes and one fp32 scale a row:
+ *   scale = max(f32(max|x| / 127), 2^-126),  code = x / scale to the nearest integer, ties to even (decided exactly).
+ * A row that holds an infinity or a NaN gets scale NaN and codes 0, so that all of its products are NaN. */
+int tbv_step_quantize_i8(signed char* codes, size_t code_stride, float* scale, const void* x, size_t x_stride,
+                         size_t rows, size_t hidden, int dtype, void* stream);
+
+/* out[m, n] = T(float(sum over k of x[m, k] * w[n, k]) * x_scale[m] * w_scale[n] + bias[n])
+ * x: m rows of k int8, w: n rows of k int8 (a linear layer's weight as stored); the sum is exact in int32 (hence the
+ * largest k), the rest fp32, rounded once to `dtype`.  x_scales is m or 1 (one scale for all rows), w_scales n or 1;
+ * bias (n elements of `dtype`) may be NULL.  k = 0 gives the bias.  out must not overlap an operand.
+ * Fast when x and w are 16-byte aligned and k and their strides multiples of 16; any other layout works. */
+#define TBV_MATMUL_I8_MAX_K 131071
+typedef struct {
+    void* out;
+    const signed char* x;
+    const float* x_scale;
+    const signed char* w;
+    const float* w_scale;
+    const void* bias;
+    int64_t out_stride, x_stride, w_stride;
+    int64_t m, n, k;
+    int64_t x_scales, w_scales;
+    int64_t dtype;
+} tbv_matmul_i8;
+int tbv_step_matmul_i8(const tbv_matmul_i8* call, void* stream);
+
+/* Rotary positions of the query and key heads of batch x tokens positions:
+ *   angle = positions[b, t] * freqs[i],  c = scale * cos(angle),  s = scale * sin(angle), negated for the inverse
+ *   (y1, y2) = (x1 * c - x2 * s, x2 * c + x1 * s)  for the pairs (i, i + rot/2), or (2i, 2i + 1) when interleaved,
+ * of the first `rot` elements (even, <= head) of each head, the others copied.  freqs: rot/2 fp64 values; positions:
+ * int64 (pos64 != 0) or int32, any sign; a stride of 0 shares them over the batch.  The angle is formed in fp64, the
+ * rest in fp32, rounded once.  The inverse is the transpose: the backward pass of a forward call with the same scale.
+ * out may be in itself with the same strides (in place); otherwise an output overlaps neither input.  heads = 0 leaves
+ * q or k out. */
+typedef struct {
+    void* out;
+    const void* in;
+    int64_t heads;
+    int64_t in_batch, in_token, in_head, out_batch, out_token, out_head;
+} tbv_rotary_heads;
+typedef struct {
+    tbv_rotary_heads q, k;
+    const void* positions;
+    const double* freqs;
+    int64_t pos_batch, pos_token;
+    int64_t batch, tokens, head, rot;
+    int64_t dtype, pos64, interleaved, inverse;
+    float scale;
+} tbv_rotary;
+int tbv_step_rotary(const tbv_rotary* call, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

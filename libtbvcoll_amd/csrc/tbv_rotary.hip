@@ -1,0 +1,241 @@
+// Query and key heads turned by their positions (rotary positions), in place or into outputs of their own.
+//
+//   angle = position * freqs[i],  c = scale cos(angle),  s = scale sin(angle)   (s = -s for the inverse)
+//   (y1, y2) = (x1 c - x2 s, x2 c + x1 s)   for the pairs (i, i + rot/2) or, interleaved, (2i, 2i + 1)
+//
+// of the first `rot` elements of a head; the rest is copied.  The inverse is the transpose of the rotation, so it is
+// the backward pass of a forward call with the same `scale`.  The angle is formed and reduced to a fraction of a turn
+// in fp64 (positions of a million lose 16 of fp32's 24 bits to whole turns); everything after it is fp32, the result
+// is rounded once to the storage type.
+// No counterpart in the reference: it is what lies between the product that follows its all-reduce and the attention.
+#include <hip/hip_runtime.h>
+#include <stdio.h>
+
+#include <utility>
+
+#include "../../include/tbvcoll.h"
+#include "tbv_device.h"
+
+namespace tbv {
+
+namespace {
+
+struct RotHeads {
+    void* out; const void* in;
+    unsigned heads;
+    ptrdiff_t in_batch, in_token, in_head, out_batch, out_token, out_head;
+};
+struct RotArgs {
+    RotHeads h[2];                              // query, key
+    const void* positions; const double* freqs;
+    ptrdiff_t pos_batch, pos_token;
+    unsigned tokens, head, half, pos64;
+    float scale;
+    int inverse;
+};
+
+template <int DT> __device__ __forceinline__ float rot_load(const void* p, ptrdiff_t i)
+{
+    if (DT == 0) return ((const float*)p)[i];
+    if (DT == 1) return (float)((const _Float16*)p)[i];
+    return __uint_as_float((uint32_t)((const uint16_t*)p)[i] << 16);
+}
+template <int DT> __device__ __forceinline__ void rot_store(void* p, ptrdiff_t i, float v)
+{
+    if (DT == 0) ((float*)p)[i] = v;
+    else if (DT == 1) ((_Float16*)p)[i] = (_Float16)v;
+    else ((__bf16*)p)[i] = (__bf16)v;
+}
+template <int DT> __device__ __forceinline__ void rot_copy(void* o, ptrdiff_t j, const void* p, ptrdiff_t i)
+{
+    if (DT == 0) ((uint32_t*)o)[j] = ((const uint32_t*)p)[i];
+    else ((uint16_t*)o)[j] = ((const uint16_t*)p)[i];
+}
+
+__device__ __forceinline__ void turn(const RotArgs& g, unsigned batch, unsigned token, unsigned i, float* c, float* s)
+{
+    const ptrdiff_t at = (ptrdiff_t)batch * g.pos_batch + (ptrdiff_t)token * g.pos_token;
+    const double p = g.pos64 ? (double)((const long long*)g.positions)[at] : (double)((const int*)g.positions)[at];
+    const double turns = p * g.freqs[i] * 0.15915494309189533577;       // 1 / (2 pi)
+    const float part = (float)(turns - __builtin_rint(turns));          // -1/2 .. 1/2 of a turn
+    float sn, cs;
+    sincospif(2.0f * part, &sn, &cs);
+    *c = cs * g.scale;
+    *s = (g.inverse ? -sn : sn) * g.scale;
+}
+
+template <int DT, bool INTER>
+__global__ __launch_bounds__(256) void k_rotary_any(RotArgs g)
+{
+    const unsigned token = blockIdx.x % g.tokens, batch = blockIdx.x / g.tokens;
+    const unsigned per_head = g.half + (g.head - 2 * g.half);            // pairs, then single elements to copy
+    for (int which = 0; which < 2; which++) {
+        const RotHeads& h = g.h[which];
+        const ptrdiff_t in0 = (ptrdiff_t)batch * h.in_batch + (ptrdiff_t)token * h.in_token;
+        const ptrdiff_t out0 = (ptrdiff_t)batch * h.out_batch + (ptrdiff_t)token * h.out_token;
+        for (size_t e = threadIdx.x; e < (size_t)h.heads * per_head; e += 256) {
+            const unsigned head = (unsigned)(e / per_head), i = (unsigned)(e % per_head);
+            const ptrdiff_t a = in0 + (ptrdiff_t)head * h.in_head, o = out0 + (ptrdiff_t)head * h.out_head;
+            if (i < g.half) {
+                float c, s;
+                turn(g, batch, token, i, &c, &s);
+                const unsigned j1 = INTER ? 2 * i : i, j2 = INTER ? 2 * i + 1 : i + g.half;
+                const float x1 = rot_load<DT>(h.in, a + j1), x2 = rot_load<DT>(h.in, a + j2);
+                rot_store<DT>(h.out, o + j1, x1 * c - x2 * s);
+                rot_store<DT>(h.out, o + j2, x2 * c + x1 * s);
+            } else if (h.out != h.in) {
+                rot_copy<DT>(h.out, o + g.half + i, h.in, a + g.half + i);
+            }
+        }
+    }
+}
+
+template <int DT> void launch_rot(const RotArgs& g, bool inter, unsigned blocks, hipStream_t st)
+{
+    if (inter) k_rotary_any<DT, true><<<dim3(blocks), 256, 0, st>>>(g);
+    else k_rotary_any<DT, false><<<dim3(blocks), 256, 0, st>>>(g);
+}
+
+// A tensor of `head` contiguous elements per (batch, token, head).
+struct Grid { const void* p; ptrdiff_t stride[3]; size_t count[3]; };
+
+// First and last byte a tensor of these sizes and strides reaches (strides may be negative or zero for an input).
+struct Span { uintptr_t lo, hi; };
+Span span_of(const Grid& g, size_t head, size_t esz)
+{
+    ptrdiff_t lo = 0, hi = (ptrdiff_t)head - 1;
+    for (int i = 0; i < 3; i++) { const ptrdiff_t d = g.stride[i] * (ptrdiff_t)(g.count[i] - 1); if (d < 0) lo += d; else hi += d; }
+    return {(uintptr_t)((intptr_t)g.p + lo * (ptrdiff_t)esz), (uintptr_t)((intptr_t)g.p + (hi + 1) * (ptrdiff_t)esz)};
+}
+bool meet(Span a, Span b) { return a.lo < b.hi && b.lo < a.hi; }
+
+// No two elements of an output share an address: sorted by stride, each dimension steps over all of the one before.
+bool self_overlaps(Grid g, size_t head)
+{
+    ptrdiff_t* s = g.stride;
+    size_t* n = g.count;
+    for (int i = 0; i < 3; i++) { if (s[i] < 0) s[i] = -s[i]; if (n[i] == 1) s[i] = 0; }
+    for (int i = 0; i < 3; i++) for (int j = i + 1; j < 3; j++) if (s[j] < s[i]) { std::swap(s[i], s[j]); std::swap(n[i], n[j]); }
+    ptrdiff_t reach = (ptrdiff_t)head;
+    for (int i = 0; i < 3; i++) {
+        if (n[i] == 1) continue;
+        if (s[i] < reach) return true;
+        reach += s[i] * (ptrdiff_t)(n[i] - 1);
+    }
+    return false;
+}
+
+// Whether two tensors, each free of overlaps in itself, may have an element in common: exact where their strides agree
+// (views of one packed buffer), yes where they do not and the spans cross.
+bool share(const Grid& a, Span sa, const Grid& b, Span sb, size_t head, size_t esz)
+{
+    if (!meet(sa, sb)) return false;
+    ptrdiff_t d = (intptr_t)b.p - (intptr_t)a.p;
+    if (d % (ptrdiff_t)esz) return true;
+    d /= (ptrdiff_t)esz;
+    // steps of b's index minus a's, along each dimension, largest stride first
+    struct Dim { ptrdiff_t stride, lo, hi; } dim[3];
+    for (int i = 0; i < 3; i++) {
+        if (a.count[i] > 1 && b.count[i] > 1 && a.stride[i] != b.stride[i]) return true;
+        ptrdiff_t st = a.count[i] > 1 ? a.stride[i] : b.stride[i];
+        ptrdiff_t lo = -(ptrdiff_t)(a.count[i] - 1), hi = (ptrdiff_t)(b.count[i] - 1);
+        if (st < 0) { st = -st; std::swap(lo, hi); lo = -lo; hi = -hi; }
+        dim[i] = {lo == hi ? 0 : st, lo, hi};
+    }
+    for (int i = 0; i < 3; i++) for (int j = i + 1; j < 3; j++) if (dim[j].stride > dim[i].stride) std::swap(dim[i], dim[j]);
+    // |d + sum of steps| < head for some steps?  What the smaller strides can still add bounds each step.
+    ptrdiff_t down[4], up[4];
+    down[3] = up[3] = (ptrdiff_t)head - 1;
+    for (int i = 2; i >= 0; i--) { down[i] = down[i + 1] - dim[i].lo * dim[i].stride; up[i] = up[i + 1] + dim[i].hi * dim[i].stride; }
+    struct Walk {
+        const Dim* dim; const ptrdiff_t *down, *up;
+        bool hit(ptrdiff_t d, int i) const
+        {
+            if (d > down[i] || -d > up[i]) return false;
+            if (i == 3) return true;
+            if (!dim[i].stride) return hit(d, i + 1);
+            // -up <= d + step*stride <= down of what is left
+            const ptrdiff_t st = dim[i].stride;
+            const auto floor_div = [](ptrdiff_t x, ptrdiff_t y) { return x >= 0 ? x / y : -((-x + y - 1) / y); };
+            ptrdiff_t from = -floor_div(up[i + 1] + d, st), to = floor_div(down[i + 1] - d, st);
+            if (from < dim[i].lo) from = dim[i].lo;
+            if (to > dim[i].hi) to = dim[i].hi;
+            if (to - from > 8) return true;             // strides that nest within one another leave three at most
+            for (ptrdiff_t k = from; k <= to; k++) if (hit(d + k * st, i + 1)) return true;
+            return false;
+        }
+    };
+    return Walk{dim, down, up}.hit(d, 0);
+}
+
+}  // namespace
+
+}  // namespace tbv
+
+#define ROT_FAIL(...) do { fprintf(stderr, "[tbvcoll] rotary: " __VA_ARGS__); fputc('\n', stderr); return -1; } while (0)
+
+extern "C" int tbv_step_rotary(const tbv_rotary* c, void* stream)
+{
+    using namespace tbv;
+    if (!c) ROT_FAIL("null arguments");
+    if (c->dtype < 0 || c->dtype > 2) ROT_FAIL("unknown dtype %lld", (long long)c->dtype);
+    const size_t esz = c->dtype == 0 ? 4 : 2;
+    if (c->batch < 0 || c->tokens < 0 || c->head < 0 || c->q.heads < 0 || c->k.heads < 0 || c->rot < 0) ROT_FAIL("a negative size");
+    if (c->rot % 2 || c->rot > c->head) ROT_FAIL("rot = %lld: an even part of a head of %lld", (long long)c->rot, (long long)c->head);
+    const long long most = 1 << 20;
+    if (c->head > most || c->q.heads > most || c->k.heads > most) ROT_FAIL("heads and their size are at most 2^20");
+    if (c->batch > 0x7fffffff || c->tokens > 0x7fffffff || c->batch * c->tokens > 0x7fffffff) ROT_FAIL("at most 2^31 - 1 tokens");
+    if (c->batch == 0 || c->tokens == 0 || c->head == 0) return 0;
+    RotArgs g{};
+    const tbv_rotary_heads* in[2] = {&c->q, &c->k};
+    Grid ins[2], outs[2];
+    Span spans_in[2], spans_out[2];
+    bool same[2] = {false, false};
+    for (int i = 0; i < 2; i++) {
+        const tbv_rotary_heads& h = *in[i];
+        if (h.heads == 0) continue;
+        if (!h.in || !h.out) ROT_FAIL("null buffer");
+        if (((uintptr_t)h.in % esz) || ((uintptr_t)h.out % esz)) ROT_FAIL("q, k and outputs must be aligned to their elements");
+        const int64_t far = (int64_t)1 << 56;               // elements a dimension may reach, so that no span overflows
+        const int64_t st[6] = {h.in_batch, h.in_token, h.in_head, h.out_batch, h.out_token, h.out_head};
+        const size_t n[3] = {(size_t)c->batch, (size_t)c->tokens, (size_t)h.heads};
+        for (int j = 0; j < 6; j++) if (n[j % 3] > 1 && (st[j] > far / (int64_t)(n[j % 3] - 1) || st[j] < -far / (int64_t)(n[j % 3] - 1))) ROT_FAIL("strides that reach beyond 2^56 elements");
+        ins[i] = Grid{h.in, {(ptrdiff_t)st[0], (ptrdiff_t)st[1], (ptrdiff_t)st[2]}, {n[0], n[1], n[2]}};
+        outs[i] = Grid{h.out, {(ptrdiff_t)st[3], (ptrdiff_t)st[4], (ptrdiff_t)st[5]}, {n[0], n[1], n[2]}};
+        for (int j = 0; j < 3; j++) if (n[j] == 1) ins[i].stride[j] = outs[i].stride[j] = 0;
+        if (self_overlaps(outs[i], c->head)) ROT_FAIL("an output whose elements share memory");
+        spans_in[i] = span_of(ins[i], c->head, esz);
+        spans_out[i] = span_of(outs[i], c->head, esz);
+        same[i] = h.in == h.out;
+        for (int j = 0; j < 3; j++) same[i] &= ins[i].stride[j] == outs[i].stride[j];
+        g.h[i] = RotHeads{h.out, h.in, (unsigned)h.heads, ins[i].stride[0], ins[i].stride[1], ins[i].stride[2],
+                          outs[i].stride[0], outs[i].stride[1], outs[i].stride[2]};
+    }
+    if (!c->q.heads && !c->k.heads) return 0;
+    if (c->rot && (!c->positions || !c->freqs)) ROT_FAIL("null positions or freqs");
+    if (((uintptr_t)c->positions % (c->pos64 ? 8 : 4)) || ((uintptr_t)c->freqs % 8)) ROT_FAIL("positions and freqs must be aligned to their elements");
+    // An output that is not its input is held apart from both inputs.  The two outputs, and an output in place and the
+    // other's input, may be views of one buffer (a packed projection): they must have no element in common.
+    for (int i = 0; i < 2; i++) {
+        if (!g.h[i].heads) continue;
+        const int o = 1 - i;
+        if (!same[i] && meet(spans_out[i], spans_in[i])) ROT_FAIL("an output overlaps its input without being it");
+        if (!g.h[o].heads) continue;
+        if (!same[i] && meet(spans_out[i], spans_in[o])) ROT_FAIL("an output overlaps the other input");
+        if (same[i] && share(outs[i], spans_out[i], ins[o], spans_in[o], c->head, esz)) ROT_FAIL("in place, q and k overlap");
+        if (share(outs[i], spans_out[i], outs[o], spans_out[o], c->head, esz)) ROT_FAIL("the outputs of q and k overlap");
+    }
+    g.positions = c->positions; g.freqs = c->freqs; g.pos_batch = (ptrdiff_t)c->pos_batch; g.pos_token = (ptrdiff_t)c->pos_token;
+    g.tokens = (unsigned)c->tokens; g.head = (unsigned)c->head; g.half = (unsigned)(c->rot / 2); g.pos64 = c->pos64 != 0;
+    g.scale = c->scale; g.inverse = c->inverse != 0;
+    const unsigned blocks = (unsigned)(c->batch * c->tokens);
+    hipStream_t st = (hipStream_t)stream;
+    switch (c->dtype) {
+        case 0: launch_rot<0>(g, c->interleaved != 0, blocks, st); break;
+        case 1: launch_rot<1>(g, c->interleaved != 0, blocks, st); break;
+        default: launch_rot<2>(g, c->interleaved != 0, blocks, st);
+    }
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) ROT_FAIL("launch failed: %s", hipGetErrorString(e));
+    return 0;
+}

@@ -16,12 +16,16 @@ two-rank exact/stress driver additionally has to hand over the peer's payload wi
 Additions (no counterpart in the reference): the emulated peer (`stage_peer`,
 `stage_peer_repeat`, `peer_resident`, `arrival_script`, `hold_rail`, `withhold`,
 `arrival_log`), measurement (`latency_probe`, `latencies`, `kernel_timing`, `kernel_times`,
-`hbm_probe`, `launch_floor`), `all_reduce_chunked`, `shutdown`, `lib`.
+`hbm_probe`, `launch_floor`), `all_reduce_chunked`, `shutdown`, `lib`, and the operators of the layer
+around the all-reduce, which need no `init`: `quantize_int8`, `matmul_int8`, `linear_int8_all_reduce`,
+`rotary`, `rotary_frequencies`.
 
 There is no CPU fallback: if the shared library is missing, `init` raises.
 """
 import ctypes
+import math
 import os
+import struct
 
 import torch
 
@@ -60,6 +64,8 @@ _SIGNATURES = {
     "tbv_emu_step_floor": (_I, [_SZ, _I, _PD]),
     "tbv_ar_allreduce_rmsnorm": (_I, [_VP, _VP, _VP, _VP, ctypes.c_float, _SZ, _SZ, _I, _VP]),
     "tbv_emu_run_sum_norm": (_I, [_I, _VP, _VP, _VP, _VP, _VP, ctypes.c_float, _SZ, _SZ, _I, _VP]),
+    "tbv_step_quantize_i8": (_I, [_VP, _SZ, _VP, _VP, _SZ, _SZ, _SZ, _I, _VP]),
+    "tbv_step_matmul_i8": (_I, [ctypes.c_char_p, _VP]), "tbv_step_rotary": (_I, [ctypes.c_char_p, _VP]),
     "tbv_emu_codec_image_bytes": (_SZ, [_SZ, _I]),
     "tbv_emu_run_quant": (_I, [_VP, _VP, _SZ, _I, _VP]), "tbv_emu_run_sum_quant": (_I, [_VP, _VP, _VP, _SZ, _I, _VP]),
 }
@@ -350,6 +356,224 @@ def all_reduce_rmsnorm(t: torch.Tensor, weight: torch.Tensor, eps: float, out: t
         return None
     _check(rc, "tbv_ar_allreduce_rmsnorm")
     return normed
+
+
+
+# ------------------------------------------------------------------ the layer around the all-reduce (additive)
+#
+# These need no `init` and have nothing to fall back to: a call they cannot take raises ValueError.  They run on the
+# current stream of the tensors' device.
+
+_step_lib = None
+_MATMUL = struct.Struct("6P9q")            # tbv_matmul_i8
+_ROTARY = struct.Struct("2P7q2P7q2P10qf4x")  # tbv_rotary
+
+
+def _steps():
+    global _step_lib
+    if _step_lib is None:
+        _step_lib = _lib or load()
+    return _step_lib
+
+
+def _need(ok, what):
+    if not ok:
+        raise ValueError(what)
+
+
+def _launch(fn, device, *args):
+    """Call a step function with the raw current stream of `device` as its last argument, that device being current."""
+    i = device.index
+    if i == torch.cuda.current_device():
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    else:
+        with torch.cuda.device(i):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+    if rc != 0:
+        raise RuntimeError(f"{fn.__name__} failed rc={rc}")
+
+
+def _rows(t, what):
+    """(rows, columns, row stride) of a tensor as a matrix of contiguous rows; leading dimensions are taken together."""
+    d = t.dim()
+    _need(d >= 1, f"{what} needs at least one dimension")
+    if d == 2:
+        (r, c), (s, e) = t.shape, t.stride()
+    else:
+        c, e = t.shape[-1], t.stride(-1)
+        r = math.prod(t.shape[:-1])
+        _need(d == 1 or t.is_contiguous() or t.numel() == 0, f"{what}: leading dimensions have to be contiguous")
+        s = c
+    _need(e == 1 or c <= 1, f"{what}: the last dimension has to be contiguous")
+    _need(r <= 1 or s >= c, f"{what}: rows overlap")
+    return r, c, s if r > 1 else max(s, c)
+
+
+def quantize_int8(x: torch.Tensor, codes: torch.Tensor = None, scale: torch.Tensor = None):
+    """Rows of `x` (last dimension; fp32, fp16 or bf16) as int8 codes with one fp32 scale a row:
+    scale = max(f32(max|x| / 127), 2^-126), code = x / scale to the nearest integer, ties to even.  Returns
+    (codes, scale) of shapes x.shape and x.shape[:-1], allocated when not given.  A row that holds an infinity or a
+    NaN gets scale NaN and codes 0, so that every product with it is NaN."""
+    code = _DT.get(x.dtype)
+    _need(x.is_cuda and code is not None, "x has to be a fp32, fp16 or bf16 tensor on the GPU")
+    rows, cols, xs = _rows(x, "x")
+    if codes is None:
+        codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    else:
+        _need(codes.dtype is torch.int8 and codes.shape == x.shape and codes.device == x.device, "codes has to be int8, of x's shape and device")
+    if scale is None:
+        scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    else:
+        _need(scale.dtype is torch.float32 and scale.shape == x.shape[:-1] and scale.device == x.device and scale.is_contiguous(),
+              "scale has to be contiguous fp32, of x's shape without its last dimension, on its device")
+    _, _, cs = _rows(codes, "codes")
+    if rows:
+        _launch(_steps().tbv_step_quantize_i8, x.device, codes.data_ptr(), cs, scale.data_ptr(), x.data_ptr(), xs, rows, cols, code)
+    return codes, scale
+
+
+def matmul_int8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: torch.Tensor = None,
+                out: torch.Tensor = None, dtype: torch.dtype = torch.bfloat16):
+    """x [..., k] int8 times w [n, k] int8 (a linear layer's weight as stored), a scale for each token and each channel:
+    out = dtype(float(sum) * x_scale * w_scale + bias), the sum exact in int32.  x_scale: fp32, one per row of x (any
+    shape of that many elements) or a single one; w_scale: fp32, n or one; bias: n elements of the result's type.
+    Returns `out` [..., n] (its type counts when given).  k up to 131071; fastest where k and the row strides are
+    multiples of 16 and the tensors 16-byte aligned.  There is no gradient: the weights are frozen codes."""
+    dev = x.device
+    _need(x.is_cuda and x.dtype is torch.int8 and w.dtype is torch.int8 and w.device == dev and w.dim() == 2, "x and w have to be int8 on one GPU, w a matrix")
+    m, k, xs = _rows(x, "x")
+    n, wk, ws = _rows(w, "w")
+    _need(k == wk, f"x has rows of {k} and w of {wk}")
+    _need(k <= 131071, f"k = {k}: beyond 131071 the int32 sum can overflow")
+    sx, sw = x_scale.numel(), w_scale.numel()
+    _need(x_scale.dtype is torch.float32 and x_scale.device == dev and x_scale.is_contiguous() and (sx == m or sx == 1),
+          "x_scale has to be contiguous fp32 on x's device, one for each row of x or one for all")
+    _need(w_scale.dtype is torch.float32 and w_scale.device == dev and w_scale.is_contiguous() and (sw == n or sw == 1),
+          "w_scale has to be contiguous fp32 on x's device, one for each row of w or one for all")
+    if out is None:
+        out = torch.empty(x.shape[:-1] + (n,), dtype=dtype, device=dev)
+    else:
+        _need(out.device == dev and out.shape == x.shape[:-1] + (n,), "out has to be on x's device, of x's shape with n columns")
+    code = _DT.get(out.dtype)
+    _need(code is not None, "the result is fp32, fp16 or bf16")
+    _need(bias is None or (bias.dtype is out.dtype and bias.device == dev and bias.is_contiguous() and bias.numel() == n),
+          "bias has to be n contiguous elements of the result's type on x's device")
+    _, _, os_ = _rows(out, "out")
+    if m and n:
+        _launch(_steps().tbv_step_matmul_i8, dev, _MATMUL.pack(
+            out.data_ptr(), x.data_ptr(), x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), 0 if bias is None else bias.data_ptr(),
+            os_, xs, ws, m, n, k, sx, sw, code))
+    return out
+
+
+def linear_int8_all_reduce(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tensor, bias: torch.Tensor = None, out: torch.Tensor = None):
+    """The row-parallel linear layer of a tensor-parallel pair with int8 weights: this rank's columns of the activations
+    `x` (fp32, fp16 or bf16) as int8 rows, times this rank's columns of the weight, SUM with the peer's partial result
+    (bias: on one rank only).  Returns the sum in x's type, or None when the library does not take the all-reduce (not
+    initialised, over the cap): the caller then runs its own layer."""
+    _need(x.is_cuda and x.dim() >= 1 and w.dim() == 2, "x has to be on the GPU and w a matrix")
+    n = w.shape[0]
+    if _lib is None or x.numel() // max(1, x.shape[-1]) * n * x.element_size() > _cap:
+        return None
+    _need(out is None or (out.dtype is x.dtype and out.is_contiguous()), "out has to be contiguous and of x's type")
+    codes, scale = quantize_int8(x)
+    out = matmul_int8(codes, scale, w, w_scale, bias=bias, out=out, dtype=x.dtype)
+    return out if all_reduce(out) else None
+
+
+def rotary_frequencies(rot: int, base: float = 10000.0, factor: float = 1.0, method: str = "linear", context: int = 0,
+                       low: float = 1.0, high: float = 32.0, device="cuda"):
+    """(freqs, scale) for `rotary`: freqs[i] = base^(-2i/rot), fp64, rot/2 of them, stretched by `factor` for contexts
+    longer than the `context` positions a model was trained on:
+
+      "linear"   every frequency divided by factor (positions interpolated);
+      "base"     the base raised to base * factor^(rot / (rot - 2)): the slowest frequency is divided by factor, the
+                 fastest kept;
+      "bands"    a frequency that turns at least `high` times within `context` is kept, one that turns at most `low`
+                 times is divided by factor, in between the two are mixed linearly in the number of turns;
+      "ramp"     as "bands", but mixed linearly in the frequency's index between the indices that turn `high` and `low`
+                 times (rounded outwards), and scale = 0.1 ln(factor) + 1 for the longer softmax.
+
+    scale is 1 except for "ramp"."""
+    _need(rot >= 2 and rot % 2 == 0, "rot has to be even and at least 2")
+    _need(base > 1.0 and factor >= 1.0, "base has to be above 1 and factor at least 1")
+    i = torch.arange(rot // 2, dtype=torch.float64)
+    scale = 1.0
+    if method == "base":
+        if rot > 2:
+            base = base * factor ** (rot / (rot - 2))
+        freqs = base ** (-2.0 * i / rot)
+    else:
+        freqs = base ** (-2.0 * i / rot)
+        if method == "linear":
+            freqs = freqs / factor
+        elif method in ("bands", "ramp"):
+            _need(context > 0 and 0 < low < high, "bands and ramp need the trained context and 0 < low < high")
+            if method == "bands":
+                keep = ((context * freqs / (2 * math.pi) - low) / (high - low)).clamp(0, 1)
+            else:
+                def index(turns):
+                    return rot * math.log(context / (turns * 2 * math.pi)) / (2 * math.log(base))
+                first, last = max(math.floor(index(high)), 0), min(math.ceil(index(low)), rot - 1)
+                keep = 1 - ((i - first) / max(last - first, 1e-3)).clamp(0, 1)
+                scale = 0.1 * math.log(factor) + 1.0
+            freqs = freqs * keep + freqs / factor * (1 - keep)
+        else:
+            raise ValueError(f"unknown method {method!r}: linear, base, bands or ramp")
+    return freqs.to(device), scale
+
+
+def _heads(t, o, what, batch, tokens, head):
+    """The nine fields of tbv_rotary_heads for t ([tokens, heads, head] or [batch, tokens, heads, head]) turned into o."""
+    s, u = t.stride(), o.stride()
+    _need((s[-1] == 1 and u[-1] == 1) or head <= 1, f"{what}: the elements of a head have to be contiguous")
+    if t.dim() == 3:
+        return o.data_ptr(), t.data_ptr(), t.shape[1], 0, s[0], s[1], 0, u[0], u[1]
+    return o.data_ptr(), t.data_ptr(), t.shape[2], s[0], s[1], s[2], u[0], u[1], u[2]
+
+
+def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, scale: float = 1.0,
+           interleaved: bool = False, inverse: bool = False, q_out: torch.Tensor = None, k_out: torch.Tensor = None):
+    """Turn the heads of q and k (k may be None) by their positions, in place where no output is given.
+
+    q, k: [tokens, heads, head] or [batch, tokens, heads, head] of one type (fp32, fp16, bf16), any strides (views of a
+    packed projection, heads before tokens) with contiguous heads.  positions: int64 or int32, [tokens] or
+    [batch, tokens].  freqs: fp64, rot/2 of them (`rotary_frequencies`): the first rot elements of a head turn, the rest
+    is copied.  Pairs are (i, i + rot/2), or (2i, 2i + 1) with `interleaved`; cos and sin are multiplied by `scale`.
+    `inverse` turns back: with the outputs' gradients for q and k it is the backward pass.  Returns (q_out, k_out)."""
+    dev, d = q.device, q.dim()
+    code = _DT.get(q.dtype)
+    _need(q.is_cuda and code is not None and d in (3, 4), "q has to be fp32, fp16 or bf16 on the GPU, [tokens, heads, head] or [batch, tokens, heads, head]")
+    batch, tokens, head = (1 if d == 3 else q.shape[0]), q.shape[-3], q.shape[-1]
+    if q_out is None:
+        q_out = q
+    else:
+        _need(q_out.dtype is q.dtype and q_out.device == dev and q_out.shape == q.shape, "q_out has to be of q's type, device and shape")
+    hq = _heads(q, q_out, "q", batch, tokens, head)
+    if k is None:
+        _need(k_out is None, "k_out without k")
+        hk = (0,) * 9
+    else:
+        _need(k.dtype is q.dtype and k.device == dev and k.dim() == d and k.shape[:-2] == q.shape[:-2] and k.shape[-1] == head,
+              "k has to be of q's type and device and differ in its heads only")
+        if k_out is None:
+            k_out = k
+        else:
+            _need(k_out.dtype is k.dtype and k_out.device == dev and k_out.shape == k.shape, "k_out has to be of k's type, device and shape")
+        hk = _heads(k, k_out, "k", batch, tokens, head)
+    pt = positions.dtype
+    _need(positions.device == dev and (pt is torch.int64 or pt is torch.int32), "positions have to be int64 or int32 on q's device")
+    if positions.dim() == 1:
+        _need(positions.shape[0] == tokens, f"{positions.shape[0]} positions for {tokens} tokens")
+        pb, ps = 0, positions.stride(0)
+    else:
+        _need(positions.dim() == 2 and d == 4 and positions.shape == q.shape[:2], "positions have to be [tokens] or [batch, tokens]")
+        pb, ps = positions.stride()
+    _need(freqs.dtype is torch.float64 and freqs.device == dev and freqs.dim() == 1 and freqs.is_contiguous() and 2 * freqs.shape[0] <= head,
+          "freqs has to be contiguous fp64 on q's device, at most half a head long")
+    _launch(_steps().tbv_step_rotary, dev, _ROTARY.pack(*hq, *hk, positions.data_ptr(), freqs.data_ptr(), pb, ps, batch, tokens, head,
+                                                        2 * freqs.shape[0], code, pt is torch.int64, interleaved, inverse, scale))
+    return q_out, k_out
 
 
 def shutdown():

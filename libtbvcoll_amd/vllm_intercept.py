@@ -118,6 +118,14 @@ class Intercept:
         normed = (x * torch.rsqrt(x.pow(2).mean(-1, keepdim=True) + eps)).to(reduced.dtype) * weight
         return reduced, normed
 
+    def row_linear_int8(self, group, input_, weight, weight_scale, bias=None):
+        """A row-parallel linear layer with int8 weights, as it stands in front of every tensor-parallel all-reduce:
+        this rank's activations as int8 rows, their product with this rank's columns of the weight (int8, a scale for
+        each output channel; bias on one rank only), and the group's all-reduce of the partial results, which goes the
+        way every other all-reduce goes (library or original)."""
+        codes, scale = self.lib.quantize_int8(input_)
+        return self._all_reduce(group, self.lib.matmul_int8(codes, scale, weight, weight_scale, bias=bias, dtype=input_.dtype))
+
     def report(self):
         """Counters plus the library's per-call averages (resets the latter), as the reference prints at the end."""
         r = dict(self.counters)
