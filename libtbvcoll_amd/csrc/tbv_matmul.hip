@@ -89,10 +89,431 @@ __global__ __launch_bounds__(256) void k_mat_any(MatArgs g)
     }
 }
 
-template <int DT> void launch_mat(const MatArgs& g, hipStream_t st)
+// ------------------------------------------------------------------ tiles in the LDS, for operands of whole 16-byte pieces
+//
+// Four waves, two by two, compute a tile of 64 TM rows of x by 64 TN rows of w; a wave holds TM x TN blocks of 32 x 32 sums.
+// A step takes 128 bytes of k, whole cache lines (two steps of 64 halve the rate of the loads).  The buffer loads write the
+// LDS directly (no registers, no address arithmetic): 128 bytes of a row are eight lanes, and the piece a lane fetches is
+// rotated by the row so that the eight rows that eight lanes of a fragment read lie in different banks.  Two buffers:
+// while step t is multiplied, step t + 1 arrives, and t + 2 is asked for as soon as the last fragment of t has been read,
+// in the middle of the step.  Fragments are read half a step ahead of the products that use them, so a step has one
+// barrier and no product waits for the LDS.
+typedef __attribute__((address_space(3))) void lds_void;
+
+template <int N> struct Int { static constexpr int value = N; };
+template <int DT> struct Out;
+template <> struct Out<0> { typedef float T; [[maybe_unused]] static constexpr int SIZE = 4; };
+template <> struct Out<1> { typedef _Float16 T; [[maybe_unused]] static constexpr int SIZE = 2; };
+template <> struct Out<2> { typedef __bf16 T; [[maybe_unused]] static constexpr int SIZE = 2; };
+
+// Which tile a block works on.  Blocks go to the eight XCDs in turn; each XCD gets a run of neighbouring tiles (bands of
+// `band` tile rows, column by column), so that the tiles its L2 serves at one time share rows of x and w.
+[[maybe_unused]] __device__ __forceinline__ void tile_of(unsigned b, unsigned tiles_m, unsigned tiles_n, unsigned band, unsigned* tm, unsigned* tn)
+{
+    const unsigned total = tiles_m * tiles_n, xcd = b & 7, q = total >> 3, r = total & 7;
+    const unsigned p = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (b >> 3);
+    const unsigned per_band = band * tiles_n, first = p / per_band * band, in = p % per_band;
+    const unsigned rows = tiles_m - first < band ? tiles_m - first : band;
+    *tm = first + in % rows;
+    *tn = in / rows;
+}
+
+template <int DT, int TM, int TN, int S, int G>
+__global__ __launch_bounds__(256 * G, TM * TN >= 8 ? 1 : 2) void k_mat_tile(MatArgs g)
+{
+#ifdef __HIP_DEVICE_COMPILE__          // (register constraints and buffer loads the host pass does not know)
+    constexpr int BM = 64 * TM, BN = 64 * TN, XS = BM * 128, WS = BN * 128, ESZ = Out<DT>::SIZE;
+    constexpr int PITCH = 32 * TN * ESZ + 16;
+    constexpr int STAGES = (S + 1) * XS + S * WS;      // one group's
+    static_assert(4 * G * 32 * PITCH + 2 * BN * 4 <= G * STAGES && (G == 1 || G * TM * TN * 16384 <= G * STAGES), "the end uses the stages' LDS");
+    __shared__ __attribute__((aligned(1024))) signed char smem[G * STAGES];
+    const unsigned tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6 & 3), group = __builtin_amdgcn_readfirstlane(tid >> 8);
+    unsigned tm, tn;
+    tile_of(blockIdx.x, (g.m + BM - 1) / BM, (g.n + BN - 1) / BN, TM >= 4 ? 4 : 8, &tm, &tn);
+    const unsigned m0 = __builtin_amdgcn_readfirstlane(tm * BM), n0 = __builtin_amdgcn_readfirstlane(tn * BN);
+
+    // the tile's rows of either operand, as a buffer of its own: the offsets of a tile fit 32 bits
+    const unsigned mrows = g.m - m0 < BM ? g.m - m0 : BM, nrows = g.n - n0 < BN ? g.n - n0 : BN;
+    const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc((void*)(g.x + (size_t)m0 * g.x_stride), 0,
+                                                                        (int)((mrows - 1) * (unsigned)g.x_stride + g.k), 0x00020000);
+    const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc((void*)(g.w + (size_t)n0 * g.w_stride), 0,
+                                                                        (int)((nrows - 1) * (unsigned)g.w_stride + g.k), 0x00020000);
+    // rows past the last one repeat it (their sums are not stored)
+    // (w's rows are rotated by bits 0, 1 and 4 of their number, since that is how they differ over eight lanes of a fragment)
+    const unsigned xpiece = (lane & 7) ^ (lane >> 3), wpiece = (lane & 7) ^ ((lane >> 3) & 3) ^ (wave >> 1) << 2;
+    unsigned xo[2 * TM], wo[2 * TN];
+#pragma unroll
+    for (int j = 0; j < 2 * TM; j++) { const unsigned r = (j * 4 + wave) * 8 + (lane >> 3); xo[j] = (r < mrows ? r : mrows - 1) * (unsigned)g.x_stride + xpiece * 16; }
+#pragma unroll
+    for (int j = 0; j < 2 * TN; j++) { const unsigned r = (j * 4 + wave) * 8 + (lane >> 3); wo[j] = (r < nrows ? r : nrows - 1) * (unsigned)g.w_stride + wpiece * 16; }
+    const unsigned steps = ((g.k + 127) / 128 + G - 1) / G;   // of each group
+    signed char* const stage = smem + group * STAGES;
+
+    // ask for a step's rows of x or w; pieces beyond k (all of a step beyond the last) lie out of the buffer's range and
+    // arrive as zeros
+    const auto fetch_x = [&](unsigned t, unsigned buf) {
+        const unsigned k0 = (t * G + group) * 128;
+        const bool past = k0 + xpiece * 16 >= g.k;
+#pragma unroll
+        for (int j = 0; j < 2 * TM; j++) __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (lds_void*)(stage + buf * XS + (j * 4 + wave) * 1024), 16, past ? 0x80000000u : xo[j], k0, 0, 0);
+    };
+    const auto fetch_w = [&](unsigned t, unsigned buf) {
+        const unsigned k0 = (t * G + group) * 128;
+        const bool past = k0 + wpiece * 16 >= g.k;
+#pragma unroll
+        for (int j = 0; j < 2 * TN; j++) __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (lds_void*)(stage + (S + 1) * XS + buf * WS + (j * 4 + wave) * 1024), 16, past ? 0x80000000u : wo[j], k0, 0, 0);
+    };
+
+    const unsigned wm = (wave & 1) * 32 * TM, wn = (wave >> 1) * 32 * TN;
+    // Where a lane's piece of a row lies, by half step and product.  Row i of a 32-row fragment of w is row
+    // 16 (i / 4 % 2) + 4 (i / 8) + i % 4 of its block: the sums a lane then holds are sixteen neighbouring columns.
+    unsigned fox[2][2], fow[2][2];
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+#pragma unroll
+        for (int q = 0; q < 2; q++) {
+            const unsigned at = ((h * 4 + q * 2 + (lane >> 5)) ^ (lane & 7)) << 4;
+            fox[h][q] = (lane & 31) * 128 + at;
+            fow[h][q] = ((lane >> 2 & 1) * 16 + (lane >> 3 & 3) * 4 + (lane & 3)) * 128 + at;
+        }
+    i32x4 fx[2][2][TM], fw[2][2][TN];
+    const auto read = [&](int h, unsigned xbuf, unsigned wbuf) {
+#pragma unroll
+        for (int q = 0; q < 2; q++) {
+#pragma unroll
+            for (int i = 0; i < TM; i++) fx[h][q][i] = *(const i32x4*)(stage + xbuf * XS + wm * 128 + i * 4096 + fox[h][q]);
+#pragma unroll
+            for (int j = 0; j < TN; j++) fw[h][q][j] = *(const i32x4*)(stage + (S + 1) * XS + wbuf * WS + wn * 128 + j * 4096 + fow[h][q]);
+        }
+    };
+    // the fragments of a half step are in registers here, not read where they are used
+    const auto hold = [&](int h) {
+#pragma unroll
+        for (int q = 0; q < 2; q++) {
+#pragma unroll
+            for (int i = 0; i < TM; i++) asm volatile("" : "+v"(fx[h][q][i]));
+#pragma unroll
+            for (int j = 0; j < TN; j++) asm volatile("" : "+v"(fw[h][q][j]));
+        }
+    };
+    i32x16 acc[TM][TN] = {};
+    const auto multiply = [&](int h) {
+#pragma unroll
+        for (int q = 0; q < 2; q++)
+#pragma unroll
+            for (int i = 0; i < TM; i++)
+#pragma unroll
+                for (int j = 0; j < TN; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fw[h][q][j], fx[h][q][i], acc[i][j], 0, 0, 0);
+    };
+    // all but the last `behind` loads of every wave have landed, every wave has its fragments in registers
+    const auto meet = [&](auto behind) {
+        constexpr int N = decltype(behind)::value;
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0x0070 | (N & 15) | (N >> 4) << 14);      // vmcnt(N) lgkmcnt(0)
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+
+#pragma unroll
+    for (int t = 0; t < S; t++) { fetch_x(t, t); fetch_w(t, t); }
+    float ws1 = 0.0f, b1 = 0.0f;                      // one column's scale and bias, for the end
+    if (tid < BN) {
+        const unsigned n = n0 + tid < g.n ? n0 + tid : g.n - 1;
+        ws1 = g.w_scale[(size_t)n * g.w_scale_step];
+        b1 = g.bias ? mat_elem<DT>(g.bias, n) : 0.0f;
+    }
+    meet(Int<(S - 1) * 2 * (TM + TN)>{});
+    read(0, 0, 0);
+    // Within a half step the loads go out first, one between two products, then the reads of the next fragments (all mixed
+    // evenly: 119 instead of 115 us at 2048 x 8192 x 8192).
+    constexpr int READS = 2 * (TM + TN);
+    unsigned x0 = 0, w0 = 0;                          // buffers of step t: t % (S + 1), t % S
+    for (unsigned t = 0; t < steps; t++) {
+        const unsigned x1 = x0 == S ? 0 : x0 + 1, w1 = w0 == S - 1 ? 0 : w0 + 1;
+        hold(0);
+        fetch_x(t + S, x0 == 0 ? S : x0 - 1);         // t - 1's buffer
+        read(1, x0, w0);
+        multiply(0);
+#pragma unroll
+        for (int i = 0; i < 2 * TM; i++) { __builtin_amdgcn_sched_group_barrier(0x010, 1, 0); __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); }
+#pragma unroll
+        for (int i = 0; i < READS; i++) { __builtin_amdgcn_sched_group_barrier(0x100, 1, 0); __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); }
+        // every fragment of t is in registers, t + 1 is in the LDS
+        meet(Int<(S - 1) * 2 * TM + (S - 2) * 2 * TN>{});
+        hold(1);
+        fetch_w(t + S, w0);
+        read(0, x1, w1);                              // (after the last step: zeros, not used)
+        multiply(1);
+#pragma unroll
+        for (int i = 0; i < 2 * TN; i++) { __builtin_amdgcn_sched_group_barrier(0x010, 1, 0); __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); }
+#pragma unroll
+        for (int i = 0; i < READS; i++) { __builtin_amdgcn_sched_group_barrier(0x100, 1, 0); __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); }
+        x0 = x1; w0 = w1;
+    }
+
+    // Results leave by strips of 32 rows of x through the wave's own part of the LDS: a lane holds sixteen neighbouring
+    // columns of a row in each block, the strip is stored in whole rows of the wave's columns.
+    typedef typename Out<DT>::T T;
+    constexpr int EPV = 16 / ESZ, VPR = 32 * TN * ESZ / 16;     // elements in 16 bytes, 16-byte vectors in a strip's row
+    typedef T TV __attribute__((ext_vector_type(EPV)));
+    meet(Int<0>{});                                   // the last loads (zeros) have landed
+    // the groups' sums are joined: each strip of 32 rows of x by one group
+    const auto owner = [](int i) { return TM % G == 0 ? i % G : 0; };
+    if constexpr (G > 1) {
+        i32x4* const sums = (i32x4*)smem + (wave * 64 + lane);
+#pragma unroll
+        for (int i = 0; i < TM; i++) {
+            if ((int)group == owner(i)) continue;
+#pragma unroll
+            for (int j = 0; j < TN; j++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) sums[((group * TM + i) * TN + j) * 1024 + r * 256] = i32x4{acc[i][j][r * 4], acc[i][j][r * 4 + 1], acc[i][j][r * 4 + 2], acc[i][j][r * 4 + 3]};
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < TM; i++) {
+            if ((int)group != owner(i)) continue;
+#pragma unroll
+            for (int o = 1; o < G; o++)
+#pragma unroll
+                for (int j = 0; j < TN; j++)
+#pragma unroll
+                    for (int r = 0; r < 4; r++) {
+                        const i32x4 v = sums[(((group + o) % G * TM + i) * TN + j) * 1024 + r * 256];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) acc[i][j][r * 4 + e] += v[e];
+                    }
+        }
+        __syncthreads();
+    }
+    float *const s_scale = (float*)smem, *const s_bias = s_scale + BN;
+    if (tid < BN) { s_scale[tid] = ws1; s_bias[tid] = b1; }
+    __syncthreads();
+    f32x4 ws[TN][4], bs[TN][4];
+#pragma unroll
+    for (int j = 0; j < TN; j++)
+#pragma unroll
+        for (int r = 0; r < 4; r++) {
+            const unsigned c = wn + j * 32 + (lane >> 5) * 16 + r * 4;
+            ws[j][r] = *(const f32x4*)(s_scale + c);
+            bs[j][r] = *(const f32x4*)(s_bias + c);
+        }
+    signed char* const strip = smem + 2 * BN * 4 + (group * 4 + wave) * 32 * PITCH;
+    const unsigned nw = n0 + wn, cols = nw >= g.n ? 0 : g.n - nw < 32 * TN ? g.n - nw : 32 * TN;
+    const bool aligned = (((uintptr_t)g.out | (g.out_stride * ESZ)) & 15) == 0, whole = aligned && cols == 32 * TN;
+#pragma unroll
+    for (int i = 0; i < TM; i++) {
+        if (G > 1 && (int)group != owner(i)) continue;
+        const unsigned ms = m0 + wm + i * 32, m = ms + (lane & 31) < g.m ? ms + (lane & 31) : g.m - 1;
+        const float xs = g.x_scale[(size_t)m * g.x_scale_step];
+#pragma unroll
+        for (int j = 0; j < TN; j++)
+#pragma unroll
+            for (int v = 0; v < 16 / EPV; v++) {
+                TV o;
+#pragma unroll
+                for (int e = 0; e < EPV; e++) {
+                    const int r = v * EPV + e;
+                    o[e] = (T)((float)acc[i][j][r] * xs * ws[j][r >> 2][r & 3] + bs[j][r >> 2][r & 3]);
+                }
+                *(TV*)(strip + (lane & 31) * PITCH + (j * 32 + (lane >> 5) * 16 + v * EPV) * ESZ) = o;
+            }
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        T* const o = (T*)g.out + (size_t)ms * g.out_stride + nw;
+        if (whole && ms + 32 <= g.m) {
+#pragma unroll
+            for (int u = 0; u < VPR / 2; u++) {
+                const unsigned v = u * 64 + lane, row = v / VPR, col = v % VPR * EPV;
+                *(u32x4*)(o + row * g.out_stride + col) = *(const u32x4*)(strip + row * PITCH + col * ESZ);
+            }
+        } else if (aligned) {                         // the last tiles: whole vectors up to the edge
+#pragma unroll 2
+            for (int u = 0; u < VPR / 2; u++) {
+                const unsigned v = u * 64 + lane, row = v / VPR, col = v % VPR * EPV;
+                if (ms + row >= g.m) continue;
+                if (col + EPV <= cols) *(u32x4*)(o + row * g.out_stride + col) = *(const u32x4*)(strip + row * PITCH + col * ESZ);
+                else for (unsigned e = col; e < cols; e++) o[row * g.out_stride + e] = *(const T*)(strip + row * PITCH + e * ESZ);
+            }
+        } else {                                      // rows that do not start on 16 bytes: an element a lane
+#pragma unroll 8
+            for (unsigned v = lane; v < 32 * 32 * TN; v += 64) {
+                const unsigned row = v / (32 * TN), col = v % (32 * TN);
+                if (ms + row < g.m && col < cols) o[row * g.out_stride + col] = *(const T*)(strip + row * PITCH + col * ESZ);
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+#endif
+}
+
+template <int DT, int TM, int TN, int S, int G> void launch_tile(const MatArgs& g, hipStream_t st)
+{
+    const size_t tiles = (size_t)((g.m + 64 * TM - 1) / (64 * TM)) * ((g.n + 64 * TN - 1) / (64 * TN));
+    k_mat_tile<DT, TM, TN, S, G><<<dim3((unsigned)tiles), 256 * G, 0, st>>>(g);
+}
+
+// ------------------------------------------------------------------ few rows of x: the weights' bytes are the work
+//
+// A block computes 16 NB columns for 16 MB rows of x; its W waves share out k in pieces of 128 bytes and their sums are
+// joined through the LDS (exact, so in any order).  Until then no wave waits for another: each has a ring of U pieces of
+// its own in the LDS, which the buffer loads fill in whole cache lines (fragments loaded straight into registers are 64
+// bytes of 16 rows a load, at half the rate: 7.1 against 6.1 us at 16 x 4096 x 4096).
+template <int DT, int MB, int NB, int W, int U>
+__global__ __launch_bounds__(64 * W) void k_mat_rows(MatArgs g)
+{
+#ifdef __HIP_DEVICE_COMPILE__
+    constexpr int ESZ = Out<DT>::SIZE, SLOT = (NB + MB) * 2048, RING = U * SLOT, LOADS = 2 * (NB + MB);
+    static_assert(RING >= MB * NB * 1024, "a wave's sums go where its ring was");
+    __shared__ __attribute__((aligned(1024))) signed char smem[W * RING];
+    const unsigned tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const unsigned n0 = blockIdx.x * 16 * NB, m0 = blockIdx.y * 16 * MB;
+    const unsigned nrows = g.n - n0 < 16 * NB ? g.n - n0 : 16 * NB, mrows = g.m - m0 < 16 * MB ? g.m - m0 : 16 * MB;
+    const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc((void*)(g.w + (size_t)n0 * g.w_stride), 0,
+                                                                        (int)((nrows - 1) * (unsigned)g.w_stride + g.k), 0x00020000);
+    const __amdgpu_buffer_rsrc_t xr = __builtin_amdgcn_make_buffer_rsrc((void*)(g.x + (size_t)m0 * g.x_stride), 0,
+                                                                        (int)((mrows - 1) * (unsigned)g.x_stride + g.k), 0x00020000);
+    // rows past the last one repeat it (their sums are not stored)
+    const unsigned at = ((lane & 7) ^ (lane >> 3)) * 16;
+    unsigned wo[2 * NB], xo[2 * MB];
+#pragma unroll
+    for (int j = 0; j < 2 * NB; j++) { const unsigned r = j * 8 + (lane >> 3); wo[j] = (r < nrows ? r : nrows - 1) * (unsigned)g.w_stride + at; }
+#pragma unroll
+    for (int i = 0; i < 2 * MB; i++) { const unsigned r = i * 8 + (lane >> 3); xo[i] = (r < mrows ? r : mrows - 1) * (unsigned)g.x_stride + at; }
+    signed char* const ring = smem + wave * RING;
+    const auto fetch = [&](unsigned piece, int u) {
+        const unsigned k0 = piece * 128;
+        const bool past = k0 + at >= g.k;                              // out of the buffer's range: zeros
+#pragma unroll
+        for (int j = 0; j < 2 * NB; j++) __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (lds_void*)(ring + u * SLOT + j * 1024), 16, past ? 0x80000000u : wo[j], k0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < 2 * MB; i++) __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (lds_void*)(ring + u * SLOT + (2 * NB + i) * 1024), 16, past ? 0x80000000u : xo[i], k0, 0, 0);
+    };
+    unsigned fo[2];
+#pragma unroll
+    for (int h = 0; h < 2; h++) fo[h] = (lane & 15) * 128 + (((h * 4 + (lane >> 4)) ^ (lane & 7)) << 4);
+    i32x4 acc[MB][NB] = {};
+    const unsigned pieces = (g.k + 127) / 128;
+#pragma unroll
+    for (int u = 0; u < U; u++) fetch(wave + u * W, u);
+    for (unsigned p = wave; p < pieces; p += U * W) {
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            constexpr int N = (U - 1) * LOADS;
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4) << 14);      // vmcnt(N): this slot's loads have landed
+            asm volatile("" ::: "memory");
+            i32x4 fw[2][NB], fx[2][MB];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+#pragma unroll
+                for (int j = 0; j < NB; j++) fw[h][j] = *(const i32x4*)(ring + u * SLOT + j * 2048 + fo[h]);
+#pragma unroll
+                for (int i = 0; i < MB; i++) fx[h][i] = *(const i32x4*)(ring + u * SLOT + (NB + i) * 2048 + fo[h]);
+            }
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_waitcnt(0xc07f);                                  // lgkmcnt(0): and have been read
+            asm volatile("" ::: "memory");
+            fetch(p + (u + U) * W, u);
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int i = 0; i < MB; i++)
+#pragma unroll
+                    for (int j = 0; j < NB; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[h][j], fx[h][i], acc[i][j], 0, 0, 0);
+        }
+    }
+    // a lane holds columns 4 (lane / 16) .. + 3 of row lane % 16
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_waitcnt(0x0070);               // the last loads (zeros) have landed: the ring is free
+    asm volatile("" ::: "memory");
+    i32x4* const part = (i32x4*)smem;
+#pragma unroll
+    for (int i = 0; i < MB; i++)
+#pragma unroll
+        for (int j = 0; j < NB; j++) part[wave * (RING / 16) + (i * NB + j) * 64 + lane] = acc[i][j];
+    __syncthreads();
+    typedef typename Out<DT>::T T;
+    for (unsigned v = tid; v < 64 * MB * NB; v += 64 * W) {
+        const unsigned m = m0 + v / (64 * NB) * 16 + (v & 15), n = n0 + v / 64 % NB * 16 + (v >> 4 & 3) * 4;
+        if (m >= g.m) continue;
+        i32x4 sum = part[v];
+#pragma unroll
+        for (int w = 1; w < W; w++) sum += part[w * (RING / 16) + v];
+        const float xs = g.x_scale[(size_t)m * g.x_scale_step];
+        T* const o = (T*)g.out + (size_t)m * g.out_stride + n;
+        typedef T T4 __attribute__((ext_vector_type(4)));
+        T4 r;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const unsigned c = n + e < g.n ? n + e : g.n - 1;
+            r[e] = (T)((float)sum[e] * xs * g.w_scale[(size_t)c * g.w_scale_step] + (g.bias ? mat_elem<DT>(g.bias, c) : 0.0f));
+        }
+        if (n + 4 <= g.n && ((uintptr_t)o & (4 * ESZ - 1)) == 0) *(T4*)o = r;
+        else for (int e = 0; e < 4; e++) if (n + e < g.n) o[e] = r[e];
+    }
+#endif
+}
+
+template <int DT, int MB, int NB, int W, int U> void launch_rows(const MatArgs& g, hipStream_t st)
+{
+    k_mat_rows<DT, MB, NB, W, U><<<dim3((g.n + 16 * NB - 1) / (16 * NB), (g.m + 16 * MB - 1) / (16 * MB)), 64 * W, 0, st>>>(g);
+}
+
+template <int DT> void launch_any(const MatArgs& g, hipStream_t st)
 {
     const size_t tiles = (size_t)((g.m + 63) / 64) * ((g.n + 63) / 64);
     k_mat_any<DT><<<dim3((unsigned)tiles), 256, 0, st>>>(g);
+}
+
+// The kernels a product of whole 16-byte pieces can take, as tiles: rows of x by rows of w.  What a tile costs on a CU by
+// itself was measured with 256 tiles, one for each CU, k = 4096 and weights from memory: `step` microseconds for each 128
+// bytes of k and `end` for the rest.  Larger tiles read less for each product, smaller ones fill the GPU; an estimate of
+// rounds of 256 tiles x (end + steps x step) decides.  Measured, in us, chosen one first: 16 x 4096 x 4096 16x16 5.5,
+// 32x32 6.5; 64 x 4096 x 4096 32x32 6.5, 64x64 8.9; 128 x 4096 x 4096 64x32 8.2, 64x64 9.0; 256 x 4096 x 4096 64x64 9.9,
+// 128x64 11.8; 512 x 4096 x 4096 128x64 14.4, 128x128 18.7; 1024 x 4096 x 4096 128x128 21.8, 128x64 27.4; 2048 x 4096 x 4096
+// 128x256 36.6, 256x256 44.6; 2048 x 8192 x 4096 256x256 63, 128x128 79.
+struct Tile { unsigned rows, cols; float end, step; };
+constexpr Tile kTiles[] = {
+    {16, 16, 0.7f, 0.07f}, {16, 32, 0.4f, 0.10f}, {16, 64, 0.6f, 0.20f}, {32, 32, 0.4f, 0.097f}, {64, 32, 0.5f, 0.145f},
+    {64, 64, 1.0f, 0.185f}, {128, 64, 1.5f, 0.31f}, {128, 128, 2.0f, 0.525f}, {128, 256, 4.0f, 0.93f}, {256, 256, 8.0f, 1.63f}};
+
+int pick_tile(unsigned m, unsigned n, unsigned k)
+{
+    const float steps = (float)((k + 127) / 128);
+    int best = 0;
+    float least = 0.0f;
+    for (int i = 0; i < (int)(sizeof kTiles / sizeof *kTiles); i++) {
+        const Tile& t = kTiles[i];
+        const size_t tm = ((size_t)m + t.rows - 1) / t.rows, tn = ((size_t)n + t.cols - 1) / t.cols;
+        if (tm > 65535 && i < 5) continue;            // the small tiles' grids have the rows of x in y
+        const float us = (float)((tm * tn + 255) / 256) * (t.end + steps * t.step);
+        if (least == 0.0f || us < least) { best = i; least = us; }
+    }
+    return best;
+}
+
+template <int DT> void launch_mat(const MatArgs& g, hipStream_t st)
+{
+    // whole 16-byte pieces, and tiles whose offsets fit 31 bits
+    const bool pieces = g.k > 0 && (((uintptr_t)g.x | (uintptr_t)g.w | g.x_stride | g.w_stride | g.k) & 15) == 0 &&
+                        g.x_stride <= (1u << 22) && g.w_stride <= (1u << 22);
+    if (!pieces) return launch_any<DT>(g, st);
+    switch (pick_tile(g.m, g.n, g.k)) {
+        case 0: return launch_rows<DT, 1, 1, 16, 2>(g, st);
+        case 1: return launch_rows<DT, 1, 2, 8, 2>(g, st);
+        case 2: return launch_rows<DT, 1, 4, 8, 2>(g, st);
+        case 3: return launch_rows<DT, 2, 2, 4, 2>(g, st);
+        case 4: return launch_rows<DT, 4, 2, 8, 1>(g, st);
+        case 5: return launch_tile<DT, 1, 1, 3, 2>(g, st);
+        case 6: return launch_tile<DT, 2, 1, 2, 2>(g, st);
+        case 7: return launch_tile<DT, 2, 2, 2, 1>(g, st);
+        case 8: return launch_tile<DT, 2, 4, 2, 1>(g, st);
+        default: return launch_tile<DT, 4, 4, 2, 1>(g, st);
+    }
 }
 
 }  // namespace
