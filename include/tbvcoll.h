@@ -154,8 +154,15 @@ int tbv_step_noalloc(void* out, const void* local, const void* received, void* b
 /* Rows of `hidden` elements of `dtype` to int8 codes and one fp32 scale a row:
  *   scale = max(f32(max|x| / 127), 2^-126),  code = x / scale to the nearest integer, ties to even (decided exactly).
  * A row that holds an infinity or a NaN gets scale NaN and codes 0, so that all of its products are NaN. */
-int tbv_step_quantize_i8(signed char* codes, size_t code_stride, float* scale, const void* x, size_t x_stride,
-                         size_t rows, size_t hidden, int dtype, void* stream);
+typedef struct {
+    signed char* codes;
+    float* scale;
+    const void* x;
+    int64_t code_stride, x_stride;
+    int64_t rows, hidden;
+    int64_t dtype;
+} tbv_quantize_i8;
+int tbv_step_quantize_i8(const tbv_quantize_i8* call, void* stream);
 
 /* out[m, n] = T(float(sum over k of x[m, k] * w[n, k]) * x_scale[m] * w_scale[n] + bias[n])
  * x: m rows of k int8, w: n rows of k int8 (a linear layer's weight as stored); the sum is exact in int32 (hence the

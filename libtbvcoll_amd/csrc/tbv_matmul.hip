@@ -543,8 +543,8 @@ extern "C" int tbv_step_matmul_i8(const tbv_matmul_i8* c, void* stream)
     if (!c->out || !c->x_scale || !c->w_scale || (c->k && (!c->x || !c->w))) MAT_FAIL("null buffer");
     if ((c->x_scales != 1 && c->x_scales != c->m) || (c->w_scales != 1 && c->w_scales != c->n)) MAT_FAIL("one scale, or one for each row");
     if ((c->m > 1 && (c->out_stride < c->n || c->x_stride < c->k)) || (c->n > 1 && c->w_stride < c->k)) MAT_FAIL("row strides shorter than a row");
-    const int64_t far = (int64_t)1 << 40;
-    if (c->out_stride > far || c->x_stride > far || c->w_stride > far) MAT_FAIL("row strides beyond 2^40");
+    const int64_t far = (int64_t)1 << 30;              // with 2^31 rows: no extent overflows
+    if ((c->m > 1 && (c->out_stride > far || c->x_stride > far)) || (c->n > 1 && c->w_stride > far)) MAT_FAIL("row strides beyond 2^30");
     if (((uintptr_t)c->out % esz) || ((uintptr_t)c->bias % esz) || ((uintptr_t)c->x_scale % 4) || ((uintptr_t)c->w_scale % 4)) MAT_FAIL("out, bias and scales must be aligned to their elements");
     const size_t tiles = ((size_t)c->m + 63) / 64 * (((size_t)c->n + 63) / 64);
     if (tiles > 0x7fffffffu) MAT_FAIL("%lld x %lld results are too many for one launch", (long long)c->m, (long long)c->n);

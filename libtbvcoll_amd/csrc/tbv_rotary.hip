@@ -11,6 +11,7 @@
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 
+#include <type_traits>
 #include <utility>
 
 #include "../../include/tbvcoll.h"
@@ -90,10 +91,140 @@ __global__ __launch_bounds__(256) void k_rotary_any(RotArgs g)
     }
 }
 
-template <int DT> void launch_rot(const RotArgs& g, bool inter, unsigned blocks, hipStream_t st)
+// Everything a multiple of 16 bytes: heads, their strides, the turned part, and in the half layout half of it.  A block
+// turns `z` tokens: its threads first form the tokens' cosines and sines in the LDS, one pair a thread (in fp64 and by
+// sincospi they would be several times the work of turning a head, were each head to form its own), then take 16
+// bytes of a head at a time: x runs over a head's vectors, y over the heads of q and k, z over the tokens, so no index is divided.
+// The first vectors are asked for before the angles are formed, which hides the way from memory.
+template <int DT> struct Lanes {                      // 16 bytes as fp32 and back, rounded to nearest even
+    static constexpr int N = 8;
+    static __device__ __forceinline__ void unpack(u32x4 v, float* f)
+    {
+        if (DT == 1) {
+            const f16x8 h = __builtin_bit_cast(f16x8, v);
+#pragma unroll
+            for (int i = 0; i < 8; i++) f[i] = (float)h[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++) { f[2 * i] = __uint_as_float(v[i] << 16); f[2 * i + 1] = __uint_as_float(v[i] & 0xffff0000u); }
+        }
+    }
+    static __device__ __forceinline__ u32x4 pack(const float* f)
+    {
+        typedef typename std::conditional<DT == 1, _Float16, __bf16>::type T;
+        typedef T T8 __attribute__((ext_vector_type(8)));
+        T8 o;
+#pragma unroll
+        for (int i = 0; i < 8; i++) o[i] = (T)f[i];
+        return __builtin_bit_cast(u32x4, o);
+    }
+};
+template <> struct Lanes<0> {
+    static constexpr int N = 4;
+    static __device__ __forceinline__ void unpack(u32x4 v, float* f)
+    {
+#pragma unroll
+        for (int i = 0; i < 4; i++) f[i] = __uint_as_float(v[i]);
+    }
+    static __device__ __forceinline__ u32x4 pack(const float* f)
+    {
+        return u32x4{__float_as_uint(f[0]), __float_as_uint(f[1]), __float_as_uint(f[2]), __float_as_uint(f[3])};
+    }
+};
+
+constexpr unsigned kRotPairs = 4096;                  // cosines and sines of a block: 32 KiB of LDS
+
+template <int DT, bool INTER>
+__global__ __launch_bounds__(512) void k_rotary(RotArgs g, unsigned total)
 {
-    if (inter) k_rotary_any<DT, true><<<dim3(blocks), 256, 0, st>>>(g);
-    else k_rotary_any<DT, false><<<dim3(blocks), 256, 0, st>>>(g);
+    constexpr unsigned N = Lanes<DT>::N;
+    extern __shared__ float2 turns[];                 // [z][half]
+    const unsigned tid = (threadIdx.z * blockDim.y + threadIdx.y) * blockDim.x + threadIdx.x;
+    const unsigned row = blockIdx.x * blockDim.z + threadIdx.z;           // batch and token
+    const unsigned token = row % g.tokens, batch = row / g.tokens;
+    const unsigned units = INTER ? 2 * g.half / N : g.half / N;           // of a head: single vectors, or pairs of them
+    const unsigned heads = g.h[0].heads + g.h[1].heads;
+    const bool mine = row < total && threadIdx.y < heads && threadIdx.x < units;
+    const char* in = nullptr;
+    char* out = nullptr;
+    constexpr ptrdiff_t ESZ = 16 / N;
+    const auto place = [&](unsigned head) {           // where a head starts
+        const bool key = head >= g.h[0].heads;
+        const RotHeads& h = g.h[key];
+        const ptrdiff_t at = key ? head - g.h[0].heads : head;
+        in = (const char*)h.in + ((ptrdiff_t)batch * h.in_batch + (ptrdiff_t)token * h.in_token + at * h.in_head) * ESZ;
+        out = (char*)h.out + ((ptrdiff_t)batch * h.out_batch + (ptrdiff_t)token * h.out_token + at * h.out_head) * ESZ;
+    };
+    u32x4 a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
+    const unsigned apart = g.half * ESZ;              // bytes between the halves
+    const auto load = [&](unsigned i) {
+        a = *(const u32x4*)(in + i * 16);
+        if (!INTER) b = *(const u32x4*)(in + i * 16 + apart);
+    };
+    if (mine) { place(threadIdx.y); load(threadIdx.x); }
+    const unsigned threads = blockDim.x * blockDim.y * blockDim.z;
+    for (unsigned e = tid; e < g.half * blockDim.z; e += threads) {
+        const unsigned z = e / g.half, r = blockIdx.x * blockDim.z + z;
+        float c, s;
+        if (r < total) { turn(g, r / g.tokens, r % g.tokens, e - z * g.half, &c, &s); turns[e] = make_float2(c, s); }
+    }
+    __syncthreads();
+    if (row >= total) return;
+    const float2* const t = turns + threadIdx.z * g.half;
+    for (unsigned head = threadIdx.y; head < heads; head += blockDim.y) {
+        if (head != threadIdx.y || !mine) place(head);
+        for (unsigned i = threadIdx.x; i < units; i += blockDim.x) {
+            if (head != threadIdx.y || i != threadIdx.x) load(i);
+            float x[N], y[N];
+            Lanes<DT>::unpack(a, x);
+            if (INTER) {
+#pragma unroll
+                for (unsigned e = 0; e < N / 2; e++) {
+                    const float2 w = t[i * (N / 2) + e];
+                    y[2 * e] = x[2 * e] * w.x - x[2 * e + 1] * w.y;
+                    y[2 * e + 1] = x[2 * e + 1] * w.x + x[2 * e] * w.y;
+                }
+                *(u32x4*)(out + i * 16) = Lanes<DT>::pack(y);
+            } else {
+                float p[N], q[N];
+                Lanes<DT>::unpack(b, y);
+#pragma unroll
+                for (unsigned e = 0; e < N; e++) {
+                    const float2 w = t[i * N + e];
+                    p[e] = x[e] * w.x - y[e] * w.y;
+                    q[e] = y[e] * w.x + x[e] * w.y;
+                }
+                *(u32x4*)(out + i * 16) = Lanes<DT>::pack(p);
+                *(u32x4*)(out + i * 16 + apart) = Lanes<DT>::pack(q);
+            }
+        }
+        if (out != in)
+            for (unsigned i = 2 * g.half / N + threadIdx.x; i < g.head / N; i += blockDim.x) *(u32x4*)(out + i * 16) = *(const u32x4*)(in + i * 16);
+    }
+}
+
+template <int DT> void launch_rot(const RotArgs& g, bool inter, unsigned total, hipStream_t st)
+{
+    constexpr unsigned N = Lanes<DT>::N, ESZ = 16 / N;
+    bool pieces = g.head % N == 0 && (inter ? 2 * g.half % N == 0 : g.half % N == 0) && g.half <= kRotPairs;
+    for (const RotHeads& h : g.h)
+        if (h.heads) pieces &= ((((uintptr_t)h.in | (uintptr_t)h.out) | (uintptr_t)((h.in_batch | h.in_token | h.in_head | h.out_batch | h.out_token | h.out_head) * (ptrdiff_t)ESZ)) & 15) == 0;
+    if (!pieces) {
+        if (inter) k_rotary_any<DT, true><<<dim3(total), 256, 0, st>>>(g);
+        else k_rotary_any<DT, false><<<dim3(total), 256, 0, st>>>(g);
+        return;
+    }
+    const unsigned units = inter ? 2 * g.half / N : g.half / N, heads = g.h[0].heads + g.h[1].heads;
+    const unsigned x = units < 1 ? 1 : units > 256 ? 256 : units;
+    const unsigned y = heads < 512 / x ? heads : 512 / x;
+    // small heads of many tokens: more than one token to a block, as long as the GPU is filled
+    unsigned z = 256 / (x * y);
+    while (z > 1 && (total / z < 1024 || g.half * z > kRotPairs)) z--;
+    if (z < 1) z = 1;
+    const dim3 grid((total + z - 1) / z), block(x, y, z);
+    const size_t lds = (size_t)g.half * z * sizeof(float2);
+    if (inter) k_rotary<DT, true><<<grid, block, lds, st>>>(g, total);
+    else k_rotary<DT, false><<<grid, block, lds, st>>>(g, total);
 }
 
 // A tensor of `head` contiguous elements per (batch, token, head).

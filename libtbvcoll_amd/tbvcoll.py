@@ -64,7 +64,7 @@ _SIGNATURES = {
     "tbv_emu_step_floor": (_I, [_SZ, _I, _PD]),
     "tbv_ar_allreduce_rmsnorm": (_I, [_VP, _VP, _VP, _VP, ctypes.c_float, _SZ, _SZ, _I, _VP]),
     "tbv_emu_run_sum_norm": (_I, [_I, _VP, _VP, _VP, _VP, _VP, ctypes.c_float, _SZ, _SZ, _I, _VP]),
-    "tbv_step_quantize_i8": (_I, [_VP, _SZ, _VP, _VP, _SZ, _SZ, _SZ, _I, _VP]),
+    "tbv_step_quantize_i8": (_I, [ctypes.c_char_p, _VP]),
     "tbv_step_matmul_i8": (_I, [ctypes.c_char_p, _VP]), "tbv_step_rotary": (_I, [ctypes.c_char_p, _VP]),
     "tbv_emu_codec_image_bytes": (_SZ, [_SZ, _I]),
     "tbv_emu_run_quant": (_I, [_VP, _VP, _SZ, _I, _VP]), "tbv_emu_run_sum_quant": (_I, [_VP, _VP, _VP, _SZ, _I, _VP]),
@@ -362,9 +362,11 @@ def all_reduce_rmsnorm(t: torch.Tensor, weight: torch.Tensor, eps: float, out: t
 # ------------------------------------------------------------------ the layer around the all-reduce (additive)
 #
 # These need no `init` and have nothing to fall back to: a call they cannot take raises ValueError.  They run on the
-# current stream of the tensors' device.
+# current stream of the tensors' device.  A decode step makes hundreds of these calls, each on the GPU for a few
+# microseconds, so they look at every attribute once and hand the library one packed structure.
 
 _step_lib = None
+_QUANTIZE = struct.Struct("3P5q")          # tbv_quantize_i8
 _MATMUL = struct.Struct("6P9q")            # tbv_matmul_i8
 _ROTARY = struct.Struct("2P7q2P7q2P10qf4x")  # tbv_rotary
 
@@ -381,32 +383,30 @@ def _need(ok, what):
         raise ValueError(what)
 
 
-def _launch(fn, device, *args):
-    """Call a step function with the raw current stream of `device` as its last argument, that device being current."""
-    i = device.index
-    if i == torch.cuda.current_device():
-        rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+def _launch(fn, device, call):
+    """Call a step function on the raw current stream of device `device` (an index), that device being current."""
+    if device == torch._C._cuda_getDevice():
+        rc = fn(call, torch._C._cuda_getCurrentRawStream(device))
     else:
-        with torch.cuda.device(i):
-            rc = fn(*args, torch._C._cuda_getCurrentRawStream(i))
+        with torch.cuda.device(device):
+            rc = fn(call, torch._C._cuda_getCurrentRawStream(device))
     if rc != 0:
         raise RuntimeError(f"{fn.__name__} failed rc={rc}")
 
 
 def _rows(t, what):
     """(rows, columns, row stride) of a tensor as a matrix of contiguous rows; leading dimensions are taken together."""
-    d = t.dim()
-    _need(d >= 1, f"{what} needs at least one dimension")
-    if d == 2:
-        (r, c), (s, e) = t.shape, t.stride()
+    if t.dim() == 2:
+        r, c = t.shape
+        s, e = t.stride()
     else:
+        _need(t.dim() >= 1, what + " needs at least one dimension")
         c, e = t.shape[-1], t.stride(-1)
-        r = math.prod(t.shape[:-1])
-        _need(d == 1 or t.is_contiguous() or t.numel() == 0, f"{what}: leading dimensions have to be contiguous")
-        s = c
-    _need(e == 1 or c <= 1, f"{what}: the last dimension has to be contiguous")
-    _need(r <= 1 or s >= c, f"{what}: rows overlap")
-    return r, c, s if r > 1 else max(s, c)
+        r, s = math.prod(t.shape[:-1]), c
+        _need(t.dim() == 1 or t.is_contiguous() or r * c == 0, what + ": leading dimensions have to be contiguous")
+    if (e != 1 and c > 1) or (s < c and r > 1):
+        raise ValueError(what + ": the last dimension has to be contiguous and rows must not overlap")
+    return r, c, s if r > 1 else c
 
 
 def quantize_int8(x: torch.Tensor, codes: torch.Tensor = None, scale: torch.Tensor = None):
@@ -414,21 +414,23 @@ def quantize_int8(x: torch.Tensor, codes: torch.Tensor = None, scale: torch.Tens
     scale = max(f32(max|x| / 127), 2^-126), code = x / scale to the nearest integer, ties to even.  Returns
     (codes, scale) of shapes x.shape and x.shape[:-1], allocated when not given.  A row that holds an infinity or a
     NaN gets scale NaN and codes 0, so that every product with it is NaN."""
-    code = _DT.get(x.dtype)
-    _need(x.is_cuda and code is not None, "x has to be a fp32, fp16 or bf16 tensor on the GPU")
+    code, dev, shape = _DT.get(x.dtype), x.get_device(), x.shape
+    if code is None or dev < 0:
+        raise ValueError("x has to be a fp32, fp16 or bf16 tensor on the GPU")
     rows, cols, xs = _rows(x, "x")
     if codes is None:
-        codes = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+        codes = torch.empty_like(x, dtype=torch.int8) if x.is_contiguous() else x.new_empty(shape, dtype=torch.int8)
+        cs = cols
     else:
-        _need(codes.dtype is torch.int8 and codes.shape == x.shape and codes.device == x.device, "codes has to be int8, of x's shape and device")
+        _need(codes.dtype is torch.int8 and codes.shape == shape and codes.get_device() == dev, "codes has to be int8, of x's shape and device")
+        cs = _rows(codes, "codes")[2]
     if scale is None:
-        scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        scale = x.new_empty(shape[:-1], dtype=torch.float32)
     else:
-        _need(scale.dtype is torch.float32 and scale.shape == x.shape[:-1] and scale.device == x.device and scale.is_contiguous(),
+        _need(scale.dtype is torch.float32 and scale.shape == shape[:-1] and scale.get_device() == dev and scale.is_contiguous(),
               "scale has to be contiguous fp32, of x's shape without its last dimension, on its device")
-    _, _, cs = _rows(codes, "codes")
     if rows:
-        _launch(_steps().tbv_step_quantize_i8, x.device, codes.data_ptr(), cs, scale.data_ptr(), x.data_ptr(), xs, rows, cols, code)
+        _launch((_step_lib or _steps()).tbv_step_quantize_i8, dev, _QUANTIZE.pack(codes.data_ptr(), scale.data_ptr(), x.data_ptr(), cs, xs, rows, cols, code))
     return codes, scale
 
 
@@ -439,30 +441,37 @@ def matmul_int8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale
     shape of that many elements) or a single one; w_scale: fp32, n or one; bias: n elements of the result's type.
     Returns `out` [..., n] (its type counts when given).  k up to 131071; fastest where k and the row strides are
     multiples of 16 and the tensors 16-byte aligned.  There is no gradient: the weights are frozen codes."""
-    dev = x.device
-    _need(x.is_cuda and x.dtype is torch.int8 and w.dtype is torch.int8 and w.device == dev and w.dim() == 2, "x and w have to be int8 on one GPU, w a matrix")
+    dev = x.get_device()
+    if dev < 0 or x.dtype is not torch.int8 or w.dtype is not torch.int8 or w.get_device() != dev or w.dim() != 2:
+        raise ValueError("x and w have to be int8 on one GPU, w a matrix")
     m, k, xs = _rows(x, "x")
     n, wk, ws = _rows(w, "w")
-    _need(k == wk, f"x has rows of {k} and w of {wk}")
-    _need(k <= 131071, f"k = {k}: beyond 131071 the int32 sum can overflow")
+    if k != wk or k > 131071:
+        raise ValueError(f"x has rows of {k} and w of {wk}: they have to be equal, and at most 131071 (beyond, the int32 sum can overflow)")
     sx, sw = x_scale.numel(), w_scale.numel()
-    _need(x_scale.dtype is torch.float32 and x_scale.device == dev and x_scale.is_contiguous() and (sx == m or sx == 1),
-          "x_scale has to be contiguous fp32 on x's device, one for each row of x or one for all")
-    _need(w_scale.dtype is torch.float32 and w_scale.device == dev and w_scale.is_contiguous() and (sw == n or sw == 1),
-          "w_scale has to be contiguous fp32 on x's device, one for each row of w or one for all")
+    if x_scale.dtype is not torch.float32 or x_scale.get_device() != dev or not x_scale.is_contiguous() or (sx != m and sx != 1):
+        raise ValueError("x_scale has to be contiguous fp32 on x's device, one for each row of x or one for all")
+    if w_scale.dtype is not torch.float32 or w_scale.get_device() != dev or not w_scale.is_contiguous() or (sw != n and sw != 1):
+        raise ValueError("w_scale has to be contiguous fp32 on x's device, one for each row of w or one for all")
     if out is None:
-        out = torch.empty(x.shape[:-1] + (n,), dtype=dtype, device=dev)
+        code, os_ = _DT.get(dtype), n
+        _need(code is not None, "the result is fp32, fp16 or bf16")
+        out = x_scale.new_empty((m, n) if x.dim() == 2 else x.shape[:-1] + (n,), dtype=dtype)
     else:
-        _need(out.device == dev and out.shape == x.shape[:-1] + (n,), "out has to be on x's device, of x's shape with n columns")
-    code = _DT.get(out.dtype)
-    _need(code is not None, "the result is fp32, fp16 or bf16")
-    _need(bias is None or (bias.dtype is out.dtype and bias.device == dev and bias.is_contiguous() and bias.numel() == n),
-          "bias has to be n contiguous elements of the result's type on x's device")
-    _, _, os_ = _rows(out, "out")
+        dtype = out.dtype
+        code = _DT.get(dtype)
+        _need(code is not None, "the result is fp32, fp16 or bf16")
+        _need(out.get_device() == dev and out.shape == x.shape[:-1] + (n,), "out has to be on x's device, of x's shape with n columns")
+        os_ = _rows(out, "out")[2]
+    if bias is None:
+        b = 0
+    else:
+        _need(bias.dtype is dtype and bias.get_device() == dev and bias.is_contiguous() and bias.numel() == n,
+              "bias has to be n contiguous elements of the result's type on x's device")
+        b = bias.data_ptr()
     if m and n:
-        _launch(_steps().tbv_step_matmul_i8, dev, _MATMUL.pack(
-            out.data_ptr(), x.data_ptr(), x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), 0 if bias is None else bias.data_ptr(),
-            os_, xs, ws, m, n, k, sx, sw, code))
+        _launch((_step_lib or _steps()).tbv_step_matmul_i8, dev, _MATMUL.pack(
+            out.data_ptr(), x.data_ptr(), x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), b, os_, xs, ws, m, n, k, sx, sw, code))
     return out
 
 
@@ -523,11 +532,17 @@ def rotary_frequencies(rot: int, base: float = 10000.0, factor: float = 1.0, met
     return freqs.to(device), scale
 
 
-def _heads(t, o, what, batch, tokens, head):
+def _heads(t, o, what):
     """The nine fields of tbv_rotary_heads for t ([tokens, heads, head] or [batch, tokens, heads, head]) turned into o."""
-    s, u = t.stride(), o.stride()
-    _need((s[-1] == 1 and u[-1] == 1) or head <= 1, f"{what}: the elements of a head have to be contiguous")
-    if t.dim() == 3:
+    s = t.stride()
+    if o is t:
+        u = s
+    else:
+        _need(o.dtype is t.dtype and o.get_device() == t.get_device() and o.shape == t.shape, what + "_out has to be of its input's type, device and shape")
+        u = o.stride()
+    if (s[-1] != 1 or u[-1] != 1) and t.shape[-1] > 1:
+        raise ValueError(what + ": the elements of a head have to be contiguous")
+    if len(s) == 3:
         return o.data_ptr(), t.data_ptr(), t.shape[1], 0, s[0], s[1], 0, u[0], u[1]
     return o.data_ptr(), t.data_ptr(), t.shape[2], s[0], s[1], s[2], u[0], u[1], u[2]
 
@@ -541,38 +556,37 @@ def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, freqs: tor
     [batch, tokens].  freqs: fp64, rot/2 of them (`rotary_frequencies`): the first rot elements of a head turn, the rest
     is copied.  Pairs are (i, i + rot/2), or (2i, 2i + 1) with `interleaved`; cos and sin are multiplied by `scale`.
     `inverse` turns back: with the outputs' gradients for q and k it is the backward pass.  Returns (q_out, k_out)."""
-    dev, d = q.device, q.dim()
-    code = _DT.get(q.dtype)
-    _need(q.is_cuda and code is not None and d in (3, 4), "q has to be fp32, fp16 or bf16 on the GPU, [tokens, heads, head] or [batch, tokens, heads, head]")
-    batch, tokens, head = (1 if d == 3 else q.shape[0]), q.shape[-3], q.shape[-1]
+    dev, shape, code = q.get_device(), q.shape, _DT.get(q.dtype)
+    d = len(shape)
+    if dev < 0 or code is None or (d != 3 and d != 4):
+        raise ValueError("q has to be fp32, fp16 or bf16 on the GPU, [tokens, heads, head] or [batch, tokens, heads, head]")
+    batch, tokens, head = 1 if d == 3 else shape[0], shape[-3], shape[-1]
     if q_out is None:
         q_out = q
-    else:
-        _need(q_out.dtype is q.dtype and q_out.device == dev and q_out.shape == q.shape, "q_out has to be of q's type, device and shape")
-    hq = _heads(q, q_out, "q", batch, tokens, head)
+    hq = _heads(q, q_out, "q")
     if k is None:
         _need(k_out is None, "k_out without k")
         hk = (0,) * 9
     else:
-        _need(k.dtype is q.dtype and k.device == dev and k.dim() == d and k.shape[:-2] == q.shape[:-2] and k.shape[-1] == head,
-              "k has to be of q's type and device and differ in its heads only")
+        ks = k.shape
+        if k.dtype is not q.dtype or k.get_device() != dev or len(ks) != d or ks[:-2] != shape[:-2] or ks[-1] != head:
+            raise ValueError("k has to be of q's type and device and differ in its heads only")
         if k_out is None:
             k_out = k
-        else:
-            _need(k_out.dtype is k.dtype and k_out.device == dev and k_out.shape == k.shape, "k_out has to be of k's type, device and shape")
-        hk = _heads(k, k_out, "k", batch, tokens, head)
-    pt = positions.dtype
-    _need(positions.device == dev and (pt is torch.int64 or pt is torch.int32), "positions have to be int64 or int32 on q's device")
-    if positions.dim() == 1:
-        _need(positions.shape[0] == tokens, f"{positions.shape[0]} positions for {tokens} tokens")
-        pb, ps = 0, positions.stride(0)
+        hk = _heads(k, k_out, "k")
+    pt, ps = positions.dtype, positions.shape
+    if positions.get_device() != dev or (pt is not torch.int64 and pt is not torch.int32):
+        raise ValueError("positions have to be int64 or int32 on q's device")
+    if len(ps) == 1 and ps[0] == tokens:
+        p0, p1 = 0, positions.stride()[0]
     else:
-        _need(positions.dim() == 2 and d == 4 and positions.shape == q.shape[:2], "positions have to be [tokens] or [batch, tokens]")
-        pb, ps = positions.stride()
-    _need(freqs.dtype is torch.float64 and freqs.device == dev and freqs.dim() == 1 and freqs.is_contiguous() and 2 * freqs.shape[0] <= head,
-          "freqs has to be contiguous fp64 on q's device, at most half a head long")
-    _launch(_steps().tbv_step_rotary, dev, _ROTARY.pack(*hq, *hk, positions.data_ptr(), freqs.data_ptr(), pb, ps, batch, tokens, head,
-                                                        2 * freqs.shape[0], code, pt is torch.int64, interleaved, inverse, scale))
+        _need(d == 4 and ps == shape[:2], "positions have to be [tokens] or [batch, tokens]")
+        p0, p1 = positions.stride()
+    rot = 2 * freqs.numel()
+    if freqs.dtype is not torch.float64 or freqs.get_device() != dev or freqs.dim() != 1 or not freqs.is_contiguous() or rot > head:
+        raise ValueError("freqs has to be contiguous fp64 on q's device, at most half a head long")
+    _launch((_step_lib or _steps()).tbv_step_rotary, dev, _ROTARY.pack(
+        *hq, *hk, positions.data_ptr(), freqs.data_ptr(), p0, p1, batch, tokens, head, rot, code, pt is torch.int64, interleaved, inverse, scale))
     return q_out, k_out
 
 

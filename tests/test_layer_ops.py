@@ -149,11 +149,11 @@ P = 1 << 20
 
 
 def quant(**kw):
-    a = dict(codes=P, code_stride=64, scale=2 * P, x=3 * P, x_stride=64, rows=4, hidden=64, dtype=2) | kw
-    return tbvcoll.load().tbv_step_quantize_i8(*a.values(), None)
+    a = dict(codes=P, scale=2 * P, x=3 * P, code_stride=64, x_stride=64, rows=4, hidden=64, dtype=2) | kw
+    return tbvcoll.load().tbv_step_quantize_i8(tbvcoll._QUANTIZE.pack(*a.values()), None)
 
 
-@pytest.mark.parametrize("kw", [dict(dtype=3), dict(dtype=-1), dict(codes=None), dict(scale=None), dict(x=None), dict(x=3 * P + 1),
+@pytest.mark.parametrize("kw", [dict(dtype=3), dict(dtype=-1), dict(codes=0), dict(scale=0), dict(x=0), dict(x=3 * P + 1), dict(rows=-1), dict(hidden=-1),
                                 dict(scale=2 * P + 2), dict(code_stride=63), dict(x_stride=63), dict(rows=1 << 31),
                                 dict(hidden=1 << 31), dict(codes=3 * P + 8), dict(scale=3 * P + 500), dict(scale=P + 16)])
 def test_refused_quantize_calls(kw, capfd):
@@ -182,7 +182,7 @@ def test_empty_calls_launch_nothing():
     assert quant(rows=0) == 0
     for kw in (dict(m=0), dict(n=0)):
         assert lib.tbv_step_matmul_i8(tbvcoll._MATMUL.pack(*(MAT | kw).values()), None) == 0
-    assert lib.tbv_step_matmul_i8(None, None) == -1 and lib.tbv_step_rotary(None, None) == -1
+    assert lib.tbv_step_matmul_i8(None, None) == -1 and lib.tbv_step_quantize_i8(None, None) == -1 and lib.tbv_step_rotary(None, None) == -1
 
 
 HEADS = ("out", "in", "heads", "in_batch", "in_token", "in_head", "out_batch", "out_token", "out_head")
