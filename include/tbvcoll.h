@@ -187,11 +187,12 @@ int tbv_step_matmul_i8(const tbv_matmul_i8* call, void* stream);
 /* Rotary positions of the query and key heads of batch x tokens positions:
  *   angle = positions[b, t] * freqs[i],  c = scale * cos(angle),  s = scale * sin(angle), negated for the inverse
  *   (y1, y2) = (x1 * c - x2 * s, x2 * c + x1 * s)  for the pairs (i, i + rot/2), or (2i, 2i + 1) when interleaved,
- * of the first `rot` elements (even, <= head) of each head, the others copied.  freqs: rot/2 fp64 values; positions:
+ * of the first `rot` elements (even, at most head and TBV_ROTARY_MAX_ROT) of each head, the others copied.  freqs: rot/2 fp64 values; positions:
  * int64 (pos64 != 0) or int32, any sign; a stride of 0 shares them over the batch.  The angle is formed in fp64, the
  * rest in fp32, rounded once.  The inverse is the transpose: the backward pass of a forward call with the same scale.
  * out may be in itself with the same strides (in place); otherwise an output overlaps neither input.  heads = 0 leaves
  * q or k out. */
+#define TBV_ROTARY_MAX_ROT 8192
 typedef struct {
     void* out;
     const void* in;

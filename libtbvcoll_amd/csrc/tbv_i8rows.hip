@@ -128,9 +128,9 @@ struct RowsArgs { signed char* codes; float* scale; const char* x; size_t code_s
 
 // A row is held in registers, read once: R rows to a block, L lanes to a row, V vectors to a lane (L > 64: one row).
 template <int DT, int L, int V>
-__global__ __launch_bounds__(L == 64 ? 256 : L) void k_quant_rows(RowsArgs g)
+__global__ __launch_bounds__(L <= 64 ? 256 : L) void k_quant_rows(RowsArgs g)
 {
-    constexpr int R = L == 64 ? 4 : 1;                // rows that share a block are waves
+    constexpr int R = L <= 64 ? 256 / L : 1;          // rows that share a block are (parts of) waves
     const unsigned lane = threadIdx.x % L, row = blockIdx.x * R + threadIdx.x / L;
     if (row >= g.rows) return;
     const char* const xr = g.x + row * g.x_stride;
@@ -141,9 +141,9 @@ __global__ __launch_bounds__(L == 64 ? 256 : L) void k_quant_rows(RowsArgs g)
 #pragma unroll
     for (int i = 0; i < V; i++) top = Vec<DT>::top(v[i], top);
 #pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) top = Vec<DT>::join(top, __shfl_xor(top, off, 64));
+    for (int off = (L < 64 ? L : 64) / 2; off >= 1; off >>= 1) top = Vec<DT>::join(top, __shfl_xor(top, off, 64));
     if (L > 64) {
-        __shared__ uint32_t wave_top[L / 64];
+        __shared__ uint32_t wave_top[L > 64 ? L / 64 : 1];
         if ((lane & 63) == 0) wave_top[lane >> 6] = top;
         __syncthreads();
 #pragma unroll
@@ -183,8 +183,12 @@ __global__ __launch_bounds__(1024) void k_quant_long(RowsArgs g)
 template <int DT> void launch_quant(const RowsArgs& g, hipStream_t st)
 {
     const unsigned vecs = (g.hidden + Vec<DT>::N - 1) / Vec<DT>::N;
-#define QUANT(L, V) k_quant_rows<DT, L, V><<<dim3(L == 64 ? (g.rows + 3) / 4 : g.rows), L == 64 ? 256 : L, 0, st>>>(g)
-    if (vecs <= 64) QUANT(64, 1);
+#define QUANT(L, V) k_quant_rows<DT, L, V><<<dim3(L <= 64 ? (g.rows + ROWS(L) - 1) / ROWS(L) : g.rows), L <= 64 ? 256 : L, 0, st>>>(g)
+#define ROWS(L) (256 / (L <= 64 ? L : 64))
+    if (vecs <= 8) QUANT(8, 1);
+    else if (vecs <= 16) QUANT(16, 1);
+    else if (vecs <= 32) QUANT(32, 1);
+    else if (vecs <= 64) QUANT(64, 1);
     else if (vecs <= 128) QUANT(64, 2);
     else if (vecs <= 256) QUANT(256, 1);
     else if (vecs <= 512) QUANT(256, 2);
@@ -193,6 +197,7 @@ template <int DT> void launch_quant(const RowsArgs& g, hipStream_t st)
     else if (vecs <= 4096) QUANT(1024, 4);
     else k_quant_long<DT><<<dim3(g.rows), 1024, 0, st>>>(g);
 #undef QUANT
+#undef ROWS
 }
 
 }  // namespace

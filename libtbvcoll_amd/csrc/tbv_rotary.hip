@@ -65,37 +65,26 @@ __device__ __forceinline__ void turn(const RotArgs& g, unsigned batch, unsigned 
     *s = (g.inverse ? -sn : sn) * g.scale;
 }
 
-template <int DT, bool INTER>
-__global__ __launch_bounds__(256) void k_rotary_any(RotArgs g)
+constexpr unsigned kRotPairs = TBV_ROTARY_MAX_ROT / 2;   // cosines and sines of a block: 32 KiB of LDS
+
+// The cosines and sines of a block's z tokens, one pair a thread.
+__device__ __forceinline__ void turn_table(const RotArgs& g, unsigned total, float2* table)
 {
-    const unsigned token = blockIdx.x % g.tokens, batch = blockIdx.x / g.tokens;
-    const unsigned per_head = g.half + (g.head - 2 * g.half);            // pairs, then single elements to copy
-    for (int which = 0; which < 2; which++) {
-        const RotHeads& h = g.h[which];
-        const ptrdiff_t in0 = (ptrdiff_t)batch * h.in_batch + (ptrdiff_t)token * h.in_token;
-        const ptrdiff_t out0 = (ptrdiff_t)batch * h.out_batch + (ptrdiff_t)token * h.out_token;
-        for (size_t e = threadIdx.x; e < (size_t)h.heads * per_head; e += 256) {
-            const unsigned head = (unsigned)(e / per_head), i = (unsigned)(e % per_head);
-            const ptrdiff_t a = in0 + (ptrdiff_t)head * h.in_head, o = out0 + (ptrdiff_t)head * h.out_head;
-            if (i < g.half) {
-                float c, s;
-                turn(g, batch, token, i, &c, &s);
-                const unsigned j1 = INTER ? 2 * i : i, j2 = INTER ? 2 * i + 1 : i + g.half;
-                const float x1 = rot_load<DT>(h.in, a + j1), x2 = rot_load<DT>(h.in, a + j2);
-                rot_store<DT>(h.out, o + j1, x1 * c - x2 * s);
-                rot_store<DT>(h.out, o + j2, x2 * c + x1 * s);
-            } else if (h.out != h.in) {
-                rot_copy<DT>(h.out, o + g.half + i, h.in, a + g.half + i);
-            }
-        }
+    const unsigned tid = (threadIdx.z * blockDim.y + threadIdx.y) * blockDim.x + threadIdx.x, threads = blockDim.x * blockDim.y * blockDim.z;
+    for (unsigned e = tid; e < g.half * blockDim.z; e += threads) {
+        const unsigned z = e / g.half, r = blockIdx.x * blockDim.z + z;
+        float c, s;
+        if (r < total) { turn(g, r / g.tokens, r % g.tokens, e - z * g.half, &c, &s); table[e] = make_float2(c, s); }
     }
+    __syncthreads();
 }
 
-// Everything a multiple of 16 bytes: heads, their strides, the turned part, and in the half layout half of it.  A block
-// turns `z` tokens: its threads first form the tokens' cosines and sines in the LDS, one pair a thread (in fp64 and by
-// sincospi they would be several times the work of turning a head, were each head to form its own), then take 16
-// bytes of a head at a time: x runs over a head's vectors, y over the heads of q and k, z over the tokens, so no index is divided.
-// The first vectors are asked for before the angles are formed, which hides the way from memory.
+// A block turns `z` tokens: its threads first form the tokens' cosines and sines in the LDS, one pair a thread (in fp64
+// and by sincospi they are several times the work of turning a head), then take 16 bytes of a head at a time: x
+// runs over a head's vectors, y over the heads of q and k, z over the tokens, so no index is divided.  The first vectors are
+// asked for before the angles are formed, which hides the way from memory.  Heads may start at any element: loads and
+// stores of 16 bytes need no alignment here; what is left of a head after whole vectors goes by elements.
+// U heads to a thread, to have more on its way at once.
 template <int DT> struct Lanes {                      // 16 bytes as fp32 and back, rounded to nearest even
     static constexpr int N = 8;
     static __device__ __forceinline__ void unpack(u32x4 v, float* f)
@@ -132,99 +121,130 @@ template <> struct Lanes<0> {
     }
 };
 
-constexpr unsigned kRotPairs = 4096;                  // cosines and sines of a block: 32 KiB of LDS
+__device__ __forceinline__ u32x4 load16(const char* p) { u32x4 v; __builtin_memcpy(&v, p, 16); return v; }
+__device__ __forceinline__ void store16(char* p, u32x4 v) { __builtin_memcpy(p, &v, 16); }
 
-template <int DT, bool INTER>
+template <int DT, bool INTER, int U>
 __global__ __launch_bounds__(512) void k_rotary(RotArgs g, unsigned total)
 {
-    constexpr unsigned N = Lanes<DT>::N;
+    constexpr unsigned N = Lanes<DT>::N, P = INTER ? N / 2 : N;          // elements and pairs of a unit
+    constexpr ptrdiff_t ESZ = 16 / N;
     extern __shared__ float2 turns[];                 // [z][half]
-    const unsigned tid = (threadIdx.z * blockDim.y + threadIdx.y) * blockDim.x + threadIdx.x;
     const unsigned row = blockIdx.x * blockDim.z + threadIdx.z;           // batch and token
     const unsigned token = row % g.tokens, batch = row / g.tokens;
-    const unsigned units = INTER ? 2 * g.half / N : g.half / N;           // of a head: single vectors, or pairs of them
-    const unsigned heads = g.h[0].heads + g.h[1].heads;
-    const bool mine = row < total && threadIdx.y < heads && threadIdx.x < units;
-    const char* in = nullptr;
-    char* out = nullptr;
-    constexpr ptrdiff_t ESZ = 16 / N;
-    const auto place = [&](unsigned head) {           // where a head starts
-        const bool key = head >= g.h[0].heads;
-        const RotHeads& h = g.h[key];
-        const ptrdiff_t at = key ? head - g.h[0].heads : head;
-        in = (const char*)h.in + ((ptrdiff_t)batch * h.in_batch + (ptrdiff_t)token * h.in_token + at * h.in_head) * ESZ;
-        out = (char*)h.out + ((ptrdiff_t)batch * h.out_batch + (ptrdiff_t)token * h.out_token + at * h.out_head) * ESZ;
+    // what a head is made of: whole units of pairs, single pairs, whole vectors to copy, single elements to copy
+    const unsigned full = g.half / P, rest = g.head - 2 * g.half, pairs = full + g.half % P, vecs = pairs + rest / N, slots = vecs + rest % N;
+    const unsigned heads = g.h[0].heads + g.h[1].heads, apart = g.half * ESZ;   // bytes between the halves
+    const char* in[U];
+    char* out[U];
+    u32x4 a[U], b[U];
+    const auto place = [&](unsigned first) {          // where this thread's heads first, first + y, ... start
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const unsigned n = first + u * blockDim.y < heads ? first + u * blockDim.y : first;
+            const bool key = n >= g.h[0].heads;
+            const RotHeads& h = g.h[key];
+            const ptrdiff_t head = key ? n - g.h[0].heads : n;
+            in[u] = (const char*)h.in + ((ptrdiff_t)batch * h.in_batch + (ptrdiff_t)token * h.in_token + head * h.in_head) * ESZ;
+            out[u] = (char*)h.out + ((ptrdiff_t)batch * h.out_batch + (ptrdiff_t)token * h.out_token + head * h.out_head) * ESZ;
+        }
     };
-    u32x4 a = {0, 0, 0, 0}, b = {0, 0, 0, 0};
-    const unsigned apart = g.half * ESZ;              // bytes between the halves
     const auto load = [&](unsigned i) {
-        a = *(const u32x4*)(in + i * 16);
-        if (!INTER) b = *(const u32x4*)(in + i * 16 + apart);
+        const unsigned at = i < full ? i * 16 : (2 * g.half + (i - pairs) * N) * ESZ;
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            a[u] = load16(in[u] + at);
+            if (!INTER && i < full) b[u] = load16(in[u] + at + apart);
+        }
     };
-    if (mine) { place(threadIdx.y); load(threadIdx.x); }
-    const unsigned threads = blockDim.x * blockDim.y * blockDim.z;
-    for (unsigned e = tid; e < g.half * blockDim.z; e += threads) {
-        const unsigned z = e / g.half, r = blockIdx.x * blockDim.z + z;
-        float c, s;
-        if (r < total) { turn(g, r / g.tokens, r % g.tokens, e - z * g.half, &c, &s); turns[e] = make_float2(c, s); }
-    }
-    __syncthreads();
+    const auto vector = [&](unsigned i) { return i < full || (i >= pairs && i < vecs); };
+    const bool mine = row < total && threadIdx.y < heads && threadIdx.x < slots;
+    if (mine) { place(threadIdx.y); if (vector(threadIdx.x)) load(threadIdx.x); }
+    turn_table(g, total, turns);
     if (row >= total) return;
     const float2* const t = turns + threadIdx.z * g.half;
-    for (unsigned head = threadIdx.y; head < heads; head += blockDim.y) {
-        if (head != threadIdx.y || !mine) place(head);
-        for (unsigned i = threadIdx.x; i < units; i += blockDim.x) {
-            if (head != threadIdx.y || i != threadIdx.x) load(i);
-            float x[N], y[N];
-            Lanes<DT>::unpack(a, x);
-            if (INTER) {
+    for (unsigned first = threadIdx.y; first < heads; first += U * blockDim.y) {
+        if (first != threadIdx.y || !mine) place(first);
+        int live = 1;                                 // heads of this thread
 #pragma unroll
-                for (unsigned e = 0; e < N / 2; e++) {
-                    const float2 w = t[i * (N / 2) + e];
-                    y[2 * e] = x[2 * e] * w.x - x[2 * e + 1] * w.y;
-                    y[2 * e + 1] = x[2 * e + 1] * w.x + x[2 * e] * w.y;
+        for (int u = 1; u < U; u++) live += first + u * blockDim.y < heads;
+        for (unsigned i = threadIdx.x; i < slots; i += blockDim.x) {
+            if (vector(i) && (first != threadIdx.y || i != threadIdx.x)) load(i);
+            if (i < full) {
+                float2 w[P];
+#pragma unroll
+                for (unsigned e = 0; e < P; e++) w[e] = t[i * P + e];
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    if (u >= live) break;
+                    float x[N], y[N], p[N], q[N];
+                    Lanes<DT>::unpack(a[u], x);
+                    if (INTER) {
+#pragma unroll
+                        for (unsigned e = 0; e < P; e++) {
+                            p[2 * e] = x[2 * e] * w[e].x - x[2 * e + 1] * w[e].y;
+                            p[2 * e + 1] = x[2 * e + 1] * w[e].x + x[2 * e] * w[e].y;
+                        }
+                        store16(out[u] + i * 16, Lanes<DT>::pack(p));
+                    } else {
+                        Lanes<DT>::unpack(b[u], y);
+#pragma unroll
+                        for (unsigned e = 0; e < P; e++) {
+                            p[e] = x[e] * w[e].x - y[e] * w[e].y;
+                            q[e] = y[e] * w[e].x + x[e] * w[e].y;
+                        }
+                        store16(out[u] + i * 16, Lanes<DT>::pack(p));
+                        store16(out[u] + i * 16 + apart, Lanes<DT>::pack(q));
+                    }
                 }
-                *(u32x4*)(out + i * 16) = Lanes<DT>::pack(y);
+            } else if (i < pairs) {
+                const unsigned e = full * P + i - full, j1 = INTER ? 2 * e : e, j2 = INTER ? 2 * e + 1 : e + g.half;
+                const float2 w = t[e];
+                float x1[U], x2[U];
+#pragma unroll
+                for (int u = 0; u < U; u++) { x1[u] = rot_load<DT>(in[u], j1); x2[u] = rot_load<DT>(in[u], j2); }
+#pragma unroll
+                for (int u = 0; u < U; u++) {
+                    if (u >= live) break;
+                    rot_store<DT>(out[u], j1, x1[u] * w.x - x2[u] * w.y);
+                    rot_store<DT>(out[u], j2, x2[u] * w.x + x1[u] * w.y);
+                }
             } else {
-                float p[N], q[N];
-                Lanes<DT>::unpack(b, y);
 #pragma unroll
-                for (unsigned e = 0; e < N; e++) {
-                    const float2 w = t[i * N + e];
-                    p[e] = x[e] * w.x - y[e] * w.y;
-                    q[e] = y[e] * w.x + x[e] * w.y;
+                for (int u = 0; u < U; u++) {
+                    if (u >= live || out[u] == in[u]) continue;
+                    if (i < vecs) store16(out[u] + (2 * g.half + (i - pairs) * N) * ESZ, a[u]);
+                    else { const unsigned e = 2 * g.half + (rest / N) * N + i - vecs; rot_copy<DT>(out[u], e, in[u], e); }
                 }
-                *(u32x4*)(out + i * 16) = Lanes<DT>::pack(p);
-                *(u32x4*)(out + i * 16 + apart) = Lanes<DT>::pack(q);
             }
         }
-        if (out != in)
-            for (unsigned i = 2 * g.half / N + threadIdx.x; i < g.head / N; i += blockDim.x) *(u32x4*)(out + i * 16) = *(const u32x4*)(in + i * 16);
     }
 }
 
 template <int DT> void launch_rot(const RotArgs& g, bool inter, unsigned total, hipStream_t st)
 {
-    constexpr unsigned N = Lanes<DT>::N, ESZ = 16 / N;
-    bool pieces = g.head % N == 0 && (inter ? 2 * g.half % N == 0 : g.half % N == 0) && g.half <= kRotPairs;
-    for (const RotHeads& h : g.h)
-        if (h.heads) pieces &= ((((uintptr_t)h.in | (uintptr_t)h.out) | (uintptr_t)((h.in_batch | h.in_token | h.in_head | h.out_batch | h.out_token | h.out_head) * (ptrdiff_t)ESZ)) & 15) == 0;
-    if (!pieces) {
-        if (inter) k_rotary_any<DT, true><<<dim3(total), 256, 0, st>>>(g);
-        else k_rotary_any<DT, false><<<dim3(total), 256, 0, st>>>(g);
-        return;
-    }
-    const unsigned units = inter ? 2 * g.half / N : g.half / N, heads = g.h[0].heads + g.h[1].heads;
-    const unsigned x = units < 1 ? 1 : units > 256 ? 256 : units;
-    const unsigned y = heads < 512 / x ? heads : 512 / x;
+    constexpr unsigned N = Lanes<DT>::N;
+    const unsigned heads = g.h[0].heads + g.h[1].heads, pairs = inter ? N / 2 : N, rest = g.head - 2 * g.half;
+    const bool copies = (g.h[0].heads && g.h[0].in != g.h[0].out) || (g.h[1].heads && g.h[1].in != g.h[1].out);
+    const unsigned slots = g.half / pairs + g.half % pairs + (copies ? rest / N + rest % N : 0);     // as in the kernel
+    const unsigned x = slots < 1 ? 1 : slots > 256 ? 256 : slots;
+    // Heads to a thread, once there are tokens enough to fill the GPU with fewer threads: four where part of a head is
+    // copied (two: 22.2 instead of 20.0 us for 8191 tokens of 20 heads of 128 fp16, 64 of them turned in interleaved pairs;
+    // 31.0 instead of 27.4 for 4096 tokens of 40 heads of 96, 46 turned), otherwise two (one: 12.6 instead of 11.3 us for 2048
+    // tokens of 40 heads of 128 bf16, 24.7 instead of 20.1 for 4096 interleaved), but one in the half layout beyond
+    // 4096 tokens (two: 36.4 instead of 34.0 us for 8192).
+    const unsigned per = total < 1024 || heads == 1 ? 1 : copies ? 4 : inter || total <= 4096 ? 2 : 1;
+    const unsigned want = (heads + per - 1) / per, y = want < 512 / x ? want : 512 / x;
     // small heads of many tokens: more than one token to a block, as long as the GPU is filled
     unsigned z = 256 / (x * y);
     while (z > 1 && (total / z < 1024 || g.half * z > kRotPairs)) z--;
     if (z < 1) z = 1;
     const dim3 grid((total + z - 1) / z), block(x, y, z);
     const size_t lds = (size_t)g.half * z * sizeof(float2);
-    if (inter) k_rotary<DT, true><<<grid, block, lds, st>>>(g, total);
-    else k_rotary<DT, false><<<grid, block, lds, st>>>(g, total);
+#define ROT(I, U) k_rotary<DT, I, U><<<grid, block, lds, st>>>(g, total)
+    if (inter) { if (per == 4) ROT(true, 4); else if (per == 2) ROT(true, 2); else ROT(true, 1); }
+    else { if (per == 4) ROT(false, 4); else if (per == 2) ROT(false, 2); else ROT(false, 1); }
+#undef ROT
 }
 
 // A tensor of `head` contiguous elements per (batch, token, head).
@@ -313,6 +333,7 @@ extern "C" int tbv_step_rotary(const tbv_rotary* c, void* stream)
     const size_t esz = c->dtype == 0 ? 4 : 2;
     if (c->batch < 0 || c->tokens < 0 || c->head < 0 || c->q.heads < 0 || c->k.heads < 0 || c->rot < 0) ROT_FAIL("a negative size");
     if (c->rot % 2 || c->rot > c->head) ROT_FAIL("rot = %lld: an even part of a head of %lld", (long long)c->rot, (long long)c->head);
+    if (c->rot > TBV_ROTARY_MAX_ROT) ROT_FAIL("rot = %lld: at most %d", (long long)c->rot, TBV_ROTARY_MAX_ROT);
     const long long most = 1 << 20;
     if (c->head > most || c->q.heads > most || c->k.heads > most) ROT_FAIL("heads and their size are at most 2^20");
     if (c->batch > 0x7fffffff || c->tokens > 0x7fffffff || c->batch * c->tokens > 0x7fffffff) ROT_FAIL("at most 2^31 - 1 tokens");

@@ -201,7 +201,7 @@ PACKED = dict(in_batch=8 * 512, in_token=512, in_head=64, out_batch=8 * 512, out
 
 
 @pytest.mark.parametrize("q,k,kw", [
-    ({}, {}, dict(dtype=3)), ({}, {}, dict(batch=-1)), ({}, {}, dict(tokens=-1)), ({}, {}, dict(rot=63)), ({}, {}, dict(rot=66)),
+    ({}, {}, dict(dtype=3)), ({}, {}, dict(batch=-1)), ({}, {}, dict(tokens=-1)), ({}, {}, dict(rot=63)), ({}, {}, dict(rot=66)), ({}, {}, dict(rot=8194, head=8194, batch=1, tokens=1)),
     ({}, {}, dict(rot=-2)), ({}, {}, dict(head=-1)), ({}, {}, dict(head=1 << 21)), ({}, {}, dict(positions=0)), ({}, {}, dict(freqs=0)),
     ({}, {}, dict(freqs=6 * P + 4)), ({}, {}, dict(positions=5 * P + 4)), ({}, {}, dict(batch=1 << 20, tokens=1 << 20)),
     (dict(heads=-1), {}, {}), (dict(out=0), {}, {}), ({"in": 0}, {}, {}), (dict(out=P + 1), {}, {}), ({}, {"in": 4 * P + 1}, {}),
