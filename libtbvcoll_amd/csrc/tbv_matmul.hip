@@ -42,51 +42,28 @@ template <int DT> __device__ __forceinline__ void mat_store(void* p, size_t i, f
     else ((__bf16*)p)[i] = (__bf16)v;
 }
 
-// 16 bytes of a row of k bytes from byte c on, zeros beyond its end; any alignment (the loads need none here).
-__device__ __forceinline__ i32x4 row_bytes(const signed char* row, unsigned c, unsigned k)
+// Bytes c .. c + 15 of a row of k bytes that starts anywhere (the loads need no alignment here), zeros beyond its end: asked
+// for with no branch, from where 16 bytes are left, and shifted into place once they have come.
+__device__ __forceinline__ i32x4 ask16(const signed char* row, unsigned c, unsigned k)
 {
     i32x4 v = {0, 0, 0, 0};
-    if (c + 16 <= k) {
-        __builtin_memcpy(&v, row + c, 16);
-    } else if (c < k) {
-        for (unsigned j = 0; j < k - c; j++) v[j >> 2] |= (int)((unsigned)(unsigned char)row[c + j] << (8 * (j & 3)));
+    if (k >= 16) {
+        __builtin_memcpy(&v, row + (c < k - 16 ? c : k - 16), 16);
+    } else if (c < k) {                               // (every lane of the grid alike)
+        for (unsigned j = 0; j < k - c && j < 16; j++) v[j >> 2] |= (int)((unsigned)(unsigned char)row[c + j] << (8 * (j & 3)));
     }
     return v;
 }
-
-// Any alignment, any strides: 64 x 64 tile, four waves of 32 x 32, 64 bytes of k a step.
-template <int DT>
-__global__ __launch_bounds__(256) void k_mat_any(MatArgs g)
+__device__ __forceinline__ i32x4 place16(i32x4 v, unsigned c, unsigned k)
 {
-    constexpr int LD = 64 + 16;                      // row pitch in the LDS: 16-byte rows of eight lanes fall into different banks
-    __shared__ __attribute__((aligned(16))) signed char sx[64 * LD], sw[64 * LD];
-    const unsigned tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const unsigned tiles_m = (g.m + 63) / 64, m0 = (blockIdx.x % tiles_m) * 64, n0 = (blockIdx.x / tiles_m) * 64;
-    const unsigned lr = tid >> 2, lc = (tid & 3) * 16;
-    const unsigned xm = m0 + lr < g.m ? m0 + lr : g.m - 1, wn = n0 + lr < g.n ? n0 + lr : g.n - 1;
-    const signed char *xr = g.x + (size_t)xm * g.x_stride, *wr = g.w + (size_t)wn * g.w_stride;
-    const unsigned wm = (wave & 1) * 32, wc = (wave >> 1) * 32;
-    i32x16 acc = {};
-    for (unsigned k0 = 0; k0 < g.k; k0 += 64) {
-        const i32x4 vx = row_bytes(xr, k0 + lc, g.k), vw = row_bytes(wr, k0 + lc, g.k);
-        __syncthreads();
-        *(i32x4*)(sx + lr * LD + lc) = vx;
-        *(i32x4*)(sw + lr * LD + lc) = vw;
-        __syncthreads();
-#pragma unroll
-        for (int h = 0; h < 2; h++) {
-            const unsigned off = (lane & 31) * LD + h * 32 + (lane >> 5) * 16;
-            acc = __builtin_amdgcn_mfma_i32_32x32x32_i8(*(const i32x4*)(sx + wm * LD + off), *(const i32x4*)(sw + wc * LD + off), acc, 0, 0, 0);
-        }
-    }
-    const unsigned n = n0 + wc + (lane & 31);
-    if (n >= g.n) return;
-    const float ws = g.w_scale[(size_t)n * g.w_scale_step], b = g.bias ? mat_elem<DT>(g.bias, n) : 0.0f;
-#pragma unroll
-    for (int r = 0; r < 16; r++) {
-        const unsigned m = m0 + wm + (r >> 2) * 8 + (lane >> 5) * 4 + (r & 3);
-        if (m < g.m) mat_store<DT>(g.out, (size_t)m * g.out_stride + n, (float)acc[r] * g.x_scale[(size_t)m * g.x_scale_step] * ws + b);
-    }
+    if (k < 16 || c + 16 <= k) return v;
+    const unsigned by = c + 16 - k;                   // bytes that come from before c
+    if (by >= 16) return i32x4{0, 0, 0, 0};
+    unsigned long long lo = (unsigned)v[0] | (unsigned long long)(unsigned)v[1] << 32, hi = (unsigned)v[2] | (unsigned long long)(unsigned)v[3] << 32;
+    if (by >= 8) { lo = hi; hi = 0; }
+    const unsigned s = (by & 7) * 8;
+    if (s) { lo = lo >> s | hi << (64 - s); hi >>= s; }
+    return i32x4{(int)(unsigned)lo, (int)(unsigned)(lo >> 32), (int)(unsigned)hi, (int)(unsigned)(hi >> 32)};
 }
 
 // ------------------------------------------------------------------ tiles in the LDS, for operands of whole 16-byte pieces
@@ -258,6 +235,12 @@ __global__ __launch_bounds__(256 * G, TM * TN >= 8 ? 1 : 2) void k_mat_tile(MatA
     typedef typename Out<DT>::T T;
     constexpr int EPV = 16 / ESZ, VPR = 32 * TN * ESZ / 16;     // elements in 16 bytes, 16-byte vectors in a strip's row
     typedef T TV __attribute__((ext_vector_type(EPV)));
+    float xs[TM];                                     // (asked for here: a load after a store to `out` would wait for it)
+#pragma unroll
+    for (int i = 0; i < TM; i++) {
+        const unsigned m = m0 + wm + i * 32 + (lane & 31);
+        xs[i] = g.x_scale[(size_t)(m < g.m ? m : g.m - 1) * g.x_scale_step];
+    }
     meet(Int<0>{});                                   // the last loads (zeros) have landed
     // the groups' sums are joined: each strip of 32 rows of x by one group
     const auto owner = [](int i) { return TM % G == 0 ? i % G : 0; };
@@ -306,8 +289,7 @@ __global__ __launch_bounds__(256 * G, TM * TN >= 8 ? 1 : 2) void k_mat_tile(MatA
 #pragma unroll
     for (int i = 0; i < TM; i++) {
         if (G > 1 && (int)group != owner(i)) continue;
-        const unsigned ms = m0 + wm + i * 32, m = ms + (lane & 31) < g.m ? ms + (lane & 31) : g.m - 1;
-        const float xs = g.x_scale[(size_t)m * g.x_scale_step];
+        const unsigned ms = m0 + wm + i * 32;
 #pragma unroll
         for (int j = 0; j < TN; j++)
 #pragma unroll
@@ -316,7 +298,7 @@ __global__ __launch_bounds__(256 * G, TM * TN >= 8 ? 1 : 2) void k_mat_tile(MatA
 #pragma unroll
                 for (int e = 0; e < EPV; e++) {
                     const int r = v * EPV + e;
-                    o[e] = (T)((float)acc[i][j][r] * xs * ws[j][r >> 2][r & 3] + bs[j][r >> 2][r & 3]);
+                    o[e] = (T)((float)acc[i][j][r] * xs[i] * ws[j][r >> 2][r & 3] + bs[j][r >> 2][r & 3]);
                 }
                 *(TV*)(strip + (lane & 31) * PITCH + (j * 32 + (lane >> 5) * 16 + v * EPV) * ESZ) = o;
             }
@@ -362,7 +344,7 @@ template <int DT, int TM, int TN, int S, int G> void launch_tile(const MatArgs& 
 // joined through the LDS (exact, so in any order).  Until then no wave waits for another: each has a ring of U pieces of
 // its own in the LDS, which the buffer loads fill in whole cache lines (fragments loaded straight into registers are 64
 // bytes of 16 rows a load, at half the rate: 7.1 against 6.1 us at 16 x 4096 x 4096).
-template <int DT, int MB, int NB, int W, int U>
+template <int DT, int MB, int NB, int W, int U, bool ANY>
 __global__ __launch_bounds__(64 * W) void k_mat_rows(MatArgs g)
 {
 #ifdef __HIP_DEVICE_COMPILE__
@@ -378,11 +360,11 @@ __global__ __launch_bounds__(64 * W) void k_mat_rows(MatArgs g)
                                                                         (int)((mrows - 1) * (unsigned)g.x_stride + g.k), 0x00020000);
     // rows past the last one repeat it (their sums are not stored)
     const unsigned at = ((lane & 7) ^ (lane >> 3)) * 16;
-    unsigned wo[2 * NB], xo[2 * MB];
+    unsigned wr_row[2 * NB], xr_row[2 * MB], wo[2 * NB], xo[2 * MB];
 #pragma unroll
-    for (int j = 0; j < 2 * NB; j++) { const unsigned r = j * 8 + (lane >> 3); wo[j] = (r < nrows ? r : nrows - 1) * (unsigned)g.w_stride + at; }
+    for (int j = 0; j < 2 * NB; j++) { const unsigned r = j * 8 + (lane >> 3); wr_row[j] = r < nrows ? r : nrows - 1; wo[j] = wr_row[j] * (unsigned)g.w_stride + at; }
 #pragma unroll
-    for (int i = 0; i < 2 * MB; i++) { const unsigned r = i * 8 + (lane >> 3); xo[i] = (r < mrows ? r : mrows - 1) * (unsigned)g.x_stride + at; }
+    for (int i = 0; i < 2 * MB; i++) { const unsigned r = i * 8 + (lane >> 3); xr_row[i] = r < mrows ? r : mrows - 1; xo[i] = xr_row[i] * (unsigned)g.x_stride + at; }
     signed char* const ring = smem + wave * RING;
     const auto fetch = [&](unsigned piece, int u) {
         const unsigned k0 = piece * 128;
@@ -397,33 +379,58 @@ __global__ __launch_bounds__(64 * W) void k_mat_rows(MatArgs g)
     for (int h = 0; h < 2; h++) fo[h] = (lane & 15) * 128 + (((h * 4 + (lane >> 4)) ^ (lane & 7)) << 4);
     i32x4 acc[MB][NB] = {};
     const unsigned pieces = (g.k + 127) / 128;
+    const auto multiply = [&](int u) {
+        i32x4 fw[2][NB], fx[2][MB];
 #pragma unroll
-    for (int u = 0; u < U; u++) fetch(wave + u * W, u);
-    for (unsigned p = wave; p < pieces; p += U * W) {
+        for (int h = 0; h < 2; h++) {
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            constexpr int N = (U - 1) * LOADS;
-            asm volatile("" ::: "memory");
-            __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4) << 14);      // vmcnt(N): this slot's loads have landed
-            asm volatile("" ::: "memory");
-            i32x4 fw[2][NB], fx[2][MB];
+            for (int j = 0; j < NB; j++) fw[h][j] = *(const i32x4*)(ring + u * SLOT + j * 2048 + fo[h]);
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
+            for (int i = 0; i < MB; i++) fx[h][i] = *(const i32x4*)(ring + u * SLOT + (NB + i) * 2048 + fo[h]);
+        }
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(0xc07f);                                      // lgkmcnt(0): the slot has been read
+        asm volatile("" ::: "memory");
 #pragma unroll
-                for (int j = 0; j < NB; j++) fw[h][j] = *(const i32x4*)(ring + u * SLOT + j * 2048 + fo[h]);
+        for (int h = 0; h < 2; h++)
 #pragma unroll
-                for (int i = 0; i < MB; i++) fx[h][i] = *(const i32x4*)(ring + u * SLOT + (NB + i) * 2048 + fo[h]);
+            for (int i = 0; i < MB; i++)
+#pragma unroll
+                for (int j = 0; j < NB; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[h][j], fx[h][i], acc[i][j], 0, 0, 0);
+    };
+    if constexpr (ANY) {
+        // rows that start anywhere: the same pieces through registers, the next one on its way during the products
+        i32x4 next[LOADS];
+        const auto load = [&](unsigned piece) {
+#pragma unroll
+            for (int j = 0; j < 2 * NB; j++) next[j] = ask16(g.w + (size_t)(n0 + wr_row[j]) * g.w_stride, piece * 128 + at, g.k);
+#pragma unroll
+            for (int i = 0; i < 2 * MB; i++) next[2 * NB + i] = ask16(g.x + (size_t)(m0 + xr_row[i]) * g.x_stride, piece * 128 + at, g.k);
+        };
+        load(wave);
+        for (unsigned p = wave; p < pieces; p += W) {
+            if ((p + 1) * 128 > g.k) {
+#pragma unroll
+                for (int l = 0; l < LOADS; l++) next[l] = place16(next[l], p * 128 + at, g.k);
             }
-            asm volatile("" ::: "memory");
-            __builtin_amdgcn_s_waitcnt(0xc07f);                                  // lgkmcnt(0): and have been read
-            asm volatile("" ::: "memory");
-            fetch(p + (u + U) * W, u);
 #pragma unroll
-            for (int h = 0; h < 2; h++)
+            for (int l = 0; l < LOADS; l++) *(i32x4*)(ring + l * 1024 + lane * 16) = next[l];
+            if (p + W < pieces) load(p + W);
+            multiply(0);
+        }
+    } else {
 #pragma unroll
-                for (int i = 0; i < MB; i++)
+        for (int u = 0; u < U; u++) fetch(wave + u * W, u);
+        for (unsigned p = wave; p < pieces; p += U * W) {
 #pragma unroll
-                    for (int j = 0; j < NB; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(fw[h][j], fx[h][i], acc[i][j], 0, 0, 0);
+            for (int u = 0; u < U; u++) {
+                constexpr int N = (U - 1) * LOADS;
+                asm volatile("" ::: "memory");
+                __builtin_amdgcn_s_waitcnt(0x0f70 | (N & 15) | (N >> 4) << 14);  // vmcnt(N): this slot's loads have landed
+                asm volatile("" ::: "memory");
+                multiply(u);
+                fetch(p + (u + U) * W, u);
+            }
         }
     }
     // a lane holds columns 4 (lane / 16) .. + 3 of row lane % 16
@@ -458,14 +465,110 @@ __global__ __launch_bounds__(64 * W) void k_mat_rows(MatArgs g)
 #endif
 }
 
-template <int DT, int MB, int NB, int W, int U> void launch_rows(const MatArgs& g, hipStream_t st)
+template <int DT, int MB, int NB, int W, int U, bool ANY = false> void launch_rows(const MatArgs& g, hipStream_t st)
 {
-    k_mat_rows<DT, MB, NB, W, U><<<dim3((g.n + 16 * NB - 1) / (16 * NB), (g.m + 16 * MB - 1) / (16 * MB)), 64 * W, 0, st>>>(g);
+    k_mat_rows<DT, MB, NB, W, U, ANY><<<dim3((g.n + 16 * NB - 1) / (16 * NB), (g.m + 16 * MB - 1) / (16 * MB)), 64 * W, 0, st>>>(g);
+}
+
+// ------------------------------------------------------------------ tiles of operands of any alignment
+//
+// 128 x 128 tile, four waves two by two, 128 bytes of k a step, laid out in the LDS as above.  Rows start anywhere, so the
+// pieces go through registers: two steps are on their way there while one is multiplied.
+template <int DT>
+__global__ __launch_bounds__(256, 2) void k_mat_any(MatArgs g)
+{
+#ifdef __HIP_DEVICE_COMPILE__
+    __shared__ __attribute__((aligned(1024))) signed char sx[2][128 * 128], sw[2][128 * 128];
+    const unsigned tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    unsigned tm, tn;
+    tile_of(blockIdx.x, (g.m + 127) / 128, (g.n + 127) / 128, 8, &tm, &tn);
+    const unsigned m0 = tm * 128, n0 = tn * 128, at = ((lane & 7) ^ (lane >> 3)) * 16;
+    const signed char *xr[4], *wr[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {                     // rows past the last one repeat it (their sums are not stored)
+        const unsigned r = (i * 4 + wave) * 8 + (lane >> 3), m = m0 + r, n = n0 + r;
+        xr[i] = g.x + (size_t)(m < g.m ? m : g.m - 1) * g.x_stride;
+        wr[i] = g.w + (size_t)(n < g.n ? n : g.n - 1) * g.w_stride;
+    }
+    const unsigned wm = (wave & 1) * 64, wn = (wave >> 1) * 64, steps = (g.k + 127) / 128;
+    i32x4 px[2][4], pw[2][4];
+    const auto load = [&](int s, unsigned t) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) { px[s][i] = ask16(xr[i], t * 128 + at, g.k); pw[s][i] = ask16(wr[i], t * 128 + at, g.k); }
+    };
+    const auto put = [&](int s, unsigned t) {         // step t into buffer t & 1 = s
+        if ((t + 1) * 128 > g.k) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) { px[s][i] = place16(px[s][i], t * 128 + at, g.k); pw[s][i] = place16(pw[s][i], t * 128 + at, g.k); }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            *(i32x4*)(sx[s] + (i * 4 + wave) * 1024 + lane * 16) = px[s][i];
+            *(i32x4*)(sw[s] + (i * 4 + wave) * 1024 + lane * 16) = pw[s][i];
+        }
+    };
+    i32x16 acc[2][2] = {};
+    const auto multiply = [&](int b) {
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const unsigned fo = (lane & 31) * 128 + (((q * 2 + (lane >> 5)) ^ (lane & 7)) << 4);
+            i32x4 fx[2], fw[2];
+#pragma unroll
+            for (int i = 0; i < 2; i++) {
+                fx[i] = *(const i32x4*)(sx[b] + (wm + i * 32) * 128 + fo);
+                fw[i] = *(const i32x4*)(sw[b] + (wn + i * 32) * 128 + fo);
+            }
+#pragma unroll
+            for (int i = 0; i < 2; i++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(fx[i], fw[j], acc[i][j], 0, 0, 0);
+        }
+    };
+    load(0, 0);
+    load(1, 1);
+    put(0, 0);
+    load(0, 2);
+    __syncthreads();
+    for (unsigned t = 0; t < steps; t += 2) {         // (an odd last step: zeros)
+        put(1, t + 1);
+        load(1, t + 3);
+        multiply(0);
+        __syncthreads();
+        put(0, t + 2);
+        load(0, t + 4);
+        multiply(1);
+        __syncthreads();
+    }
+    // (scales and bias first: a load after a store to `out` would wait for it)
+    float xs[2][16], ws[2], bias[2];
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+        const unsigned n = n0 + wn + j * 32 + (lane & 31), c = n < g.n ? n : g.n - 1;
+        ws[j] = g.w_scale[(size_t)c * g.w_scale_step];
+        bias[j] = g.bias ? mat_elem<DT>(g.bias, c) : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            const unsigned m = m0 + wm + i * 32 + (r >> 2) * 8 + (lane >> 5) * 4 + (r & 3);
+            xs[i][r] = g.x_scale[(size_t)(m < g.m ? m : g.m - 1) * g.x_scale_step];
+        }
+#pragma unroll
+    for (int i = 0; i < 2; i++)
+#pragma unroll
+        for (int r = 0; r < 16; r++)
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const unsigned n = n0 + wn + j * 32 + (lane & 31), m = m0 + wm + i * 32 + (r >> 2) * 8 + (lane >> 5) * 4 + (r & 3);
+                if (m < g.m && n < g.n) mat_store<DT>(g.out, (size_t)m * g.out_stride + n, (float)acc[i][j][r] * xs[i][r] * ws[j] + bias[j]);
+            }
+#endif
 }
 
 template <int DT> void launch_any(const MatArgs& g, hipStream_t st)
 {
-    const size_t tiles = (size_t)((g.m + 63) / 64) * ((g.n + 63) / 64);
+    const size_t tiles = (size_t)((g.m + 127) / 128) * ((g.n + 127) / 128);
     k_mat_any<DT><<<dim3((unsigned)tiles), 256, 0, st>>>(g);
 }
 
@@ -476,20 +579,26 @@ template <int DT> void launch_any(const MatArgs& g, hipStream_t st)
 // 32x32 6.5; 64 x 4096 x 4096 32x32 6.5, 64x64 8.9; 128 x 4096 x 4096 64x32 8.2, 64x64 9.0; 256 x 4096 x 4096 64x64 9.9,
 // 128x64 11.8; 512 x 4096 x 4096 128x64 14.4, 128x128 18.7; 1024 x 4096 x 4096 128x128 21.8, 128x64 27.4; 2048 x 4096 x 4096
 // 128x256 36.6, 256x256 44.6; 2048 x 8192 x 4096 256x256 63, 128x128 79.
-struct Tile { unsigned rows, cols; float end, step; };
+struct Tile { unsigned rows, cols; float end, step; bool ring; };
 constexpr Tile kTiles[] = {
-    {16, 16, 0.7f, 0.07f}, {16, 32, 0.4f, 0.10f}, {16, 64, 0.6f, 0.20f}, {32, 32, 0.4f, 0.097f}, {64, 32, 0.5f, 0.145f},
-    {64, 64, 1.0f, 0.185f}, {128, 64, 1.5f, 0.31f}, {128, 128, 2.0f, 0.525f}, {128, 256, 4.0f, 0.93f}, {256, 256, 8.0f, 1.63f}};
+    {16, 16, 0.7f, 0.07f, true}, {16, 32, 0.4f, 0.10f, true}, {16, 64, 0.6f, 0.20f, true}, {32, 32, 0.4f, 0.097f, true},
+    {64, 32, 0.5f, 0.145f, true}, {64, 64, 1.0f, 0.185f, false}, {128, 64, 1.5f, 0.31f, false}, {128, 128, 2.0f, 0.525f, false},
+    {128, 256, 4.0f, 0.93f, false}, {256, 256, 8.0f, 1.63f, false}};
+// The same for rows that start anywhere.  Measured, in us, chosen one first: 16 x 4096 x 4097 16x16 6.0, 32x32 9.0;
+// 77 x 2741 x 1111 16x32 5.9, 64x64 9.8; 64 x 4096 x 4097 32x32 8.9, 64x64 18.3; 512 x 4096 x 4097 64x64 30.1, 128x128 43.7;
+// 1024 x 4096 x 4097 128x128 44.7, 64x64 55.4.
+constexpr Tile kAnyTiles[] = {
+    {16, 16, 0.3f, 0.085f, true}, {16, 32, 0.4f, 0.14f, true}, {32, 32, 0.5f, 0.165f, true}, {64, 64, 0.8f, 0.42f, true}, {128, 128, 2.0f, 1.1f, false}};
 
-int pick_tile(unsigned m, unsigned n, unsigned k)
+template <int N> int pick_tile(const Tile (&tiles)[N], unsigned m, unsigned n, unsigned k)
 {
     const float steps = (float)((k + 127) / 128);
-    int best = 0;
+    int best = N - 1;
     float least = 0.0f;
-    for (int i = 0; i < (int)(sizeof kTiles / sizeof *kTiles); i++) {
-        const Tile& t = kTiles[i];
+    for (int i = 0; i < N; i++) {
+        const Tile& t = tiles[i];
         const size_t tm = ((size_t)m + t.rows - 1) / t.rows, tn = ((size_t)n + t.cols - 1) / t.cols;
-        if (tm > 65535 && i < 5) continue;            // the small tiles' grids have the rows of x in y
+        if (t.ring && tm > 65535) continue;           // a grid's y
         const float us = (float)((tm * tn + 255) / 256) * (t.end + steps * t.step);
         if (least == 0.0f || us < least) { best = i; least = us; }
     }
@@ -501,8 +610,16 @@ template <int DT> void launch_mat(const MatArgs& g, hipStream_t st)
     // whole 16-byte pieces, and tiles whose offsets fit 31 bits
     const bool pieces = g.k > 0 && (((uintptr_t)g.x | (uintptr_t)g.w | g.x_stride | g.w_stride | g.k) & 15) == 0 &&
                         g.x_stride <= (1u << 22) && g.w_stride <= (1u << 22);
-    if (!pieces) return launch_any<DT>(g, st);
-    switch (pick_tile(g.m, g.n, g.k)) {
+    if (!pieces) {
+        switch (pick_tile(kAnyTiles, g.m, g.n, g.k)) {
+            case 0: return launch_rows<DT, 1, 1, 8, 1, true>(g, st);
+            case 1: return launch_rows<DT, 1, 2, 8, 1, true>(g, st);
+            case 2: return launch_rows<DT, 2, 2, 8, 1, true>(g, st);
+            case 3: return launch_rows<DT, 4, 4, 4, 1, true>(g, st);
+            default: return launch_any<DT>(g, st);
+        }
+    }
+    switch (pick_tile(kTiles, g.m, g.n, g.k)) {
         case 0: return launch_rows<DT, 1, 1, 16, 2>(g, st);
         case 1: return launch_rows<DT, 1, 2, 8, 2>(g, st);
         case 2: return launch_rows<DT, 1, 4, 8, 2>(g, st);

@@ -225,7 +225,7 @@ template <int DT> void launch_rot(const RotArgs& g, bool inter, unsigned total, 
 {
     constexpr unsigned N = Lanes<DT>::N;
     const unsigned heads = g.h[0].heads + g.h[1].heads, pairs = inter ? N / 2 : N, rest = g.head - 2 * g.half;
-    const bool copies = (g.h[0].heads && g.h[0].in != g.h[0].out) || (g.h[1].heads && g.h[1].in != g.h[1].out);
+    const bool copies = rest && ((g.h[0].heads && g.h[0].in != g.h[0].out) || (g.h[1].heads && g.h[1].in != g.h[1].out));
     const unsigned slots = g.half / pairs + g.half % pairs + (copies ? rest / N + rest % N : 0);     // as in the kernel
     const unsigned x = slots < 1 ? 1 : slots > 256 ? 256 : slots;
     // Heads to a thread, once there are tokens enough to fill the GPU with fewer threads: four where part of a head is
