@@ -42,21 +42,17 @@ template <int DT> __device__ __forceinline__ void mat_store(void* p, size_t i, f
     else ((__bf16*)p)[i] = (__bf16)v;
 }
 
-// Bytes c .. c + 15 of a row of k bytes that starts anywhere (the loads need no alignment here), zeros beyond its end: asked
-// for with no branch, from where 16 bytes are left, and shifted into place once they have come.
-__device__ __forceinline__ i32x4 ask16(const signed char* row, unsigned c, unsigned k)
+// Bytes c .. c + 15 of a row of k >= 16 bytes that starts anywhere (the loads need no alignment here), zeros beyond its
+// end: asked for with no branch, from where 16 bytes are left, and shifted into place once they have come.
+[[maybe_unused]] __device__ __forceinline__ i32x4 ask16(const signed char* row, unsigned c, unsigned k)
 {
-    i32x4 v = {0, 0, 0, 0};
-    if (k >= 16) {
-        __builtin_memcpy(&v, row + (c < k - 16 ? c : k - 16), 16);
-    } else if (c < k) {                               // (every lane of the grid alike)
-        for (unsigned j = 0; j < k - c && j < 16; j++) v[j >> 2] |= (int)((unsigned)(unsigned char)row[c + j] << (8 * (j & 3)));
-    }
+    i32x4 v;
+    __builtin_memcpy(&v, row + (c < k - 16 ? c : k - 16), 16);
     return v;
 }
-__device__ __forceinline__ i32x4 place16(i32x4 v, unsigned c, unsigned k)
+[[maybe_unused]] __device__ __forceinline__ i32x4 place16(i32x4 v, unsigned c, unsigned k)
 {
-    if (k < 16 || c + 16 <= k) return v;
+    if (c + 16 <= k) return v;
     const unsigned by = c + 16 - k;                   // bytes that come from before c
     if (by >= 16) return i32x4{0, 0, 0, 0};
     unsigned long long lo = (unsigned)v[0] | (unsigned long long)(unsigned)v[1] << 32, hi = (unsigned)v[2] | (unsigned long long)(unsigned)v[3] << 32;
@@ -64,6 +60,19 @@ __device__ __forceinline__ i32x4 place16(i32x4 v, unsigned c, unsigned k)
     const unsigned s = (by & 7) * 8;
     if (s) { lo = lo >> s | hi << (64 - s); hi >>= s; }
     return i32x4{(int)(unsigned)lo, (int)(unsigned)(lo >> 32), (int)(unsigned)hi, (int)(unsigned)(hi >> 32)};
+}
+
+// k < 16: a result a thread.
+template <int DT>
+__global__ __launch_bounds__(256) void k_mat_short(MatArgs g)
+{
+    for (size_t at = (size_t)blockIdx.x * 256 + threadIdx.x; at < (size_t)g.m * g.n; at += (size_t)gridDim.x * 256) {
+        const size_t m = at / g.n, n = at % g.n;
+        int sum = 0;
+        for (unsigned k = 0; k < g.k; k++) sum += (int)g.x[m * g.x_stride + k] * (int)g.w[n * g.w_stride + k];
+        const float b = g.bias ? mat_elem<DT>(g.bias, n) : 0.0f;
+        mat_store<DT>(g.out, m * g.out_stride + n, (float)sum * g.x_scale[m * g.x_scale_step] * g.w_scale[n * g.w_scale_step] + b);
+    }
 }
 
 // ------------------------------------------------------------------ tiles in the LDS, for operands of whole 16-byte pieces
@@ -585,10 +594,10 @@ constexpr Tile kTiles[] = {
     {64, 32, 0.5f, 0.145f, true}, {64, 64, 1.0f, 0.185f, false}, {128, 64, 1.5f, 0.31f, false}, {128, 128, 2.0f, 0.525f, false},
     {128, 256, 4.0f, 0.93f, false}, {256, 256, 8.0f, 1.63f, false}};
 // The same for rows that start anywhere.  Measured, in us, chosen one first: 16 x 4096 x 4097 16x16 6.0, 32x32 9.0;
-// 77 x 2741 x 1111 16x32 5.9, 64x64 9.8; 64 x 4096 x 4097 32x32 8.9, 64x64 18.3; 512 x 4096 x 4097 64x64 30.1, 128x128 43.7;
-// 1024 x 4096 x 4097 128x128 44.7, 64x64 55.4.
+// 77 x 2741 x 1111 16x32 5.8, 64x64 9.8; 64 x 4096 x 4097 32x32 8.9, 64x64 17.6; 512 x 4096 x 4097 64x64 30.4, 128x128 36.6;
+// 1024 x 4096 x 4097 128x128 38.1, 64x64 55.3.
 constexpr Tile kAnyTiles[] = {
-    {16, 16, 0.3f, 0.085f, true}, {16, 32, 0.4f, 0.14f, true}, {32, 32, 0.5f, 0.165f, true}, {64, 64, 0.8f, 0.42f, true}, {128, 128, 2.0f, 1.1f, false}};
+    {16, 16, 0.3f, 0.085f, true}, {16, 32, 0.4f, 0.14f, true}, {32, 32, 0.5f, 0.165f, true}, {64, 64, 0.8f, 0.42f, true}, {128, 128, 3.0f, 1.05f, false}};
 
 template <int N> int pick_tile(const Tile (&tiles)[N], unsigned m, unsigned n, unsigned k)
 {
@@ -608,8 +617,13 @@ template <int N> int pick_tile(const Tile (&tiles)[N], unsigned m, unsigned n, u
 template <int DT> void launch_mat(const MatArgs& g, hipStream_t st)
 {
     // whole 16-byte pieces, and tiles whose offsets fit 31 bits
-    const bool pieces = g.k > 0 && (((uintptr_t)g.x | (uintptr_t)g.w | g.x_stride | g.w_stride | g.k) & 15) == 0 &&
+    const bool pieces = (((uintptr_t)g.x | (uintptr_t)g.w | g.x_stride | g.w_stride | g.k) & 15) == 0 &&
                         g.x_stride <= (1u << 22) && g.w_stride <= (1u << 22);
+    if (g.k < 16) {
+        const size_t blocks = ((size_t)g.m * g.n + 255) / 256;
+        k_mat_short<DT><<<dim3((unsigned)(blocks < 65536 ? blocks : 65536)), 256, 0, st>>>(g);
+        return;
+    }
     if (!pieces) {
         switch (pick_tile(kAnyTiles, g.m, g.n, g.k)) {
             case 0: return launch_rows<DT, 1, 1, 8, 1, true>(g, st);
