@@ -125,8 +125,9 @@ __global__ __launch_bounds__(256 * G, TM * TN >= 8 ? 1 : 2) void k_mat_tile(MatA
     const __amdgpu_buffer_rsrc_t wr = __builtin_amdgcn_make_buffer_rsrc((void*)(g.w + (size_t)n0 * g.w_stride), 0,
                                                                         (int)((nrows - 1) * (unsigned)g.w_stride + g.k), 0x00020000);
     // rows past the last one repeat it (their sums are not stored)
-    // (w's rows are rotated by bits 0, 1 and 4 of their number, since that is how they differ over eight lanes of a fragment)
-    const unsigned xpiece = (lane & 7) ^ (lane >> 3), wpiece = (lane & 7) ^ ((lane >> 3) & 3) ^ (wave >> 1) << 2;
+    // The LDS has 64 banks, two rows of 128 bytes: sixteen lanes of a fragment that are read together differ in bits 0 .. 3 of
+    // their row of x, and in bits 0, 1, 2 and 4 of their row of w.  Bit 0 is the half of the banks, the others turn the row.
+    const unsigned xpiece = (lane & 7) ^ (lane >> 4) ^ (wave & 1) << 2, wpiece = (lane & 7) ^ (lane >> 4) ^ (wave >> 1) << 2;
     unsigned xo[2 * TM], wo[2 * TN];
 #pragma unroll
     for (int j = 0; j < 2 * TM; j++) { const unsigned r = (j * 4 + wave) * 8 + (lane >> 3); xo[j] = (r < mrows ? r : mrows - 1) * (unsigned)g.x_stride + xpiece * 16; }
@@ -158,9 +159,9 @@ __global__ __launch_bounds__(256 * G, TM * TN >= 8 ? 1 : 2) void k_mat_tile(MatA
     for (int h = 0; h < 2; h++)
 #pragma unroll
         for (int q = 0; q < 2; q++) {
-            const unsigned at = ((h * 4 + q * 2 + (lane >> 5)) ^ (lane & 7)) << 4;
-            fox[h][q] = (lane & 31) * 128 + at;
-            fow[h][q] = ((lane >> 2 & 1) * 16 + (lane >> 3 & 3) * 4 + (lane & 3)) * 128 + at;
+            const unsigned c = h * 4 + q * 2 + (lane >> 5);
+            fox[h][q] = (lane & 31) * 128 + ((c ^ (lane >> 1 & 7)) << 4);
+            fow[h][q] = ((lane >> 2 & 1) * 16 + (lane >> 3 & 3) * 4 + (lane & 3)) * 128 + ((c ^ (lane >> 1 & 1) ^ (lane >> 3 & 1) << 1 ^ (lane >> 2 & 1) << 2) << 4);
         }
     i32x4 fx[2][2][TM], fw[2][2][TN];
     const auto read = [&](int h, unsigned xbuf, unsigned wbuf) {
@@ -212,9 +213,10 @@ __global__ __launch_bounds__(256 * G, TM * TN >= 8 ? 1 : 2) void k_mat_tile(MatA
     }
     meet(Int<(S - 1) * 2 * (TM + TN)>{});
     read(0, 0, 0);
-    // Within a half step the loads go out first, one between two products, then the reads of the next fragments (all mixed
-    // evenly: 119 instead of 115 us at 2048 x 8192 x 8192).
-    constexpr int READS = 2 * (TM + TN);
+    // Within a half step the loads go out first, in large tiles two products apart (the CU takes one in 18 cycles, and a
+    // load that has to wait holds up the products behind it), then the reads of the next fragments.  2048 x 8192 x 8192:
+    // this order 110 us, loads one product apart 114, reads before loads 121, both mixed evenly 124.
+    constexpr int READS = 2 * (TM + TN), GAP = TM * TN >= 8 ? 2 : 1;
     unsigned x0 = 0, w0 = 0;                          // buffers of step t: t % (S + 1), t % S
     for (unsigned t = 0; t < steps; t++) {
         const unsigned x1 = x0 == S ? 0 : x0 + 1, w1 = w0 == S - 1 ? 0 : w0 + 1;
@@ -223,9 +225,9 @@ __global__ __launch_bounds__(256 * G, TM * TN >= 8 ? 1 : 2) void k_mat_tile(MatA
         read(1, x0, w0);
         multiply(0);
 #pragma unroll
-        for (int i = 0; i < 2 * TM; i++) { __builtin_amdgcn_sched_group_barrier(0x010, 1, 0); __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); }
+        for (int i = 0; i < 2 * TM; i++) { __builtin_amdgcn_sched_group_barrier(0x010, 1, 0); __builtin_amdgcn_sched_group_barrier(0x008, GAP, 0); }
 #pragma unroll
-        for (int i = 0; i < READS; i++) { __builtin_amdgcn_sched_group_barrier(0x100, 1, 0); __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); }
+        for (int i = 0; i < READS / GAP; i++) { __builtin_amdgcn_sched_group_barrier(0x100, GAP, 0); __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); }
         // every fragment of t is in registers, t + 1 is in the LDS
         meet(Int<(S - 1) * 2 * TM + (S - 2) * 2 * TN>{});
         hold(1);
@@ -233,9 +235,9 @@ __global__ __launch_bounds__(256 * G, TM * TN >= 8 ? 1 : 2) void k_mat_tile(MatA
         read(0, x1, w1);                              // (after the last step: zeros, not used)
         multiply(1);
 #pragma unroll
-        for (int i = 0; i < 2 * TN; i++) { __builtin_amdgcn_sched_group_barrier(0x010, 1, 0); __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); }
+        for (int i = 0; i < 2 * TN; i++) { __builtin_amdgcn_sched_group_barrier(0x010, 1, 0); __builtin_amdgcn_sched_group_barrier(0x008, GAP, 0); }
 #pragma unroll
-        for (int i = 0; i < READS; i++) { __builtin_amdgcn_sched_group_barrier(0x100, 1, 0); __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); }
+        for (int i = 0; i < READS / GAP; i++) { __builtin_amdgcn_sched_group_barrier(0x100, GAP, 0); __builtin_amdgcn_sched_group_barrier(0x008, 1, 0); }
         x0 = x1; w0 = w1;
     }
 
@@ -491,7 +493,7 @@ __global__ __launch_bounds__(256, 2) void k_mat_any(MatArgs g)
     const unsigned tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     unsigned tm, tn;
     tile_of(blockIdx.x, (g.m + 127) / 128, (g.n + 127) / 128, 8, &tm, &tn);
-    const unsigned m0 = tm * 128, n0 = tn * 128, at = ((lane & 7) ^ (lane >> 3)) * 16;
+    const unsigned m0 = tm * 128, n0 = tn * 128, at = ((lane & 7) ^ (lane >> 4) ^ (wave & 1) << 2) * 16;
     const signed char *xr[4], *wr[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {                     // rows past the last one repeat it (their sums are not stored)
@@ -520,7 +522,7 @@ __global__ __launch_bounds__(256, 2) void k_mat_any(MatArgs g)
     const auto multiply = [&](int b) {
 #pragma unroll
         for (int q = 0; q < 4; q++) {
-            const unsigned fo = (lane & 31) * 128 + (((q * 2 + (lane >> 5)) ^ (lane & 7)) << 4);
+            const unsigned fo = (lane & 31) * 128 + (((q * 2 + (lane >> 5)) ^ (lane >> 1 & 7)) << 4);
             i32x4 fx[2], fw[2];
 #pragma unroll
             for (int i = 0; i < 2; i++) {
@@ -590,7 +592,7 @@ template <int DT> void launch_any(const MatArgs& g, hipStream_t st)
 // 128x256 36.6, 256x256 44.6; 2048 x 8192 x 4096 256x256 63, 128x128 79.
 struct Tile { unsigned rows, cols; float end, step; bool ring; };
 constexpr Tile kTiles[] = {
-    {16, 16, 0.7f, 0.07f, true}, {16, 32, 0.4f, 0.10f, true}, {16, 64, 0.6f, 0.20f, true}, {32, 32, 0.4f, 0.097f, true},
+    {16, 16, 0.7f, 0.07f, true}, {16, 32, 0.4f, 0.09f, true}, {16, 64, 0.6f, 0.18f, true}, {32, 32, 0.4f, 0.097f, true},
     {64, 32, 0.5f, 0.145f, true}, {64, 64, 1.0f, 0.185f, false}, {128, 64, 1.5f, 0.31f, false}, {128, 128, 2.0f, 0.525f, false},
     {128, 256, 4.0f, 0.93f, false}, {256, 256, 8.0f, 1.63f, false}};
 // The same for rows that start anywhere.  Measured, in us, chosen one first: 16 x 4096 x 4097 16x16 6.0, 32x32 9.0;
