@@ -11,6 +11,7 @@
 
 #include "../../include/tbvcoll.h"
 #include "tbv_device.h"
+#include "tbv_step.h"
 
 namespace tbv {
 
@@ -131,7 +132,8 @@ template <int DT, int L, int V>
 __global__ __launch_bounds__(L <= 64 ? 256 : L) void k_quant_rows(RowsArgs g)
 {
     constexpr int R = L <= 64 ? 256 / L : 1;          // rows that share a block are (parts of) waves
-    const unsigned lane = threadIdx.x % L, row = blockIdx.x * R + threadIdx.x / L;
+    const unsigned lane = threadIdx.x % L;
+    const size_t row = flat_block() * R + threadIdx.x / L;
     if (row >= g.rows) return;
     const char* const xr = g.x + row * g.x_stride;
     u32x4 v[V];
@@ -162,7 +164,8 @@ __global__ __launch_bounds__(1024) void k_quant_long(RowsArgs g)
 {
     __shared__ uint32_t wave_top[16];
     const unsigned lane = threadIdx.x, vecs = (g.hidden + Vec<DT>::N - 1) / Vec<DT>::N;
-    const size_t row = blockIdx.x;
+    const size_t row = flat_block();
+    if (row >= g.rows) return;
     const char* const xr = g.x + row * g.x_stride;
     uint32_t top = 0;
 #pragma unroll 4
@@ -183,7 +186,7 @@ __global__ __launch_bounds__(1024) void k_quant_long(RowsArgs g)
 template <int DT> void launch_quant(const RowsArgs& g, hipStream_t st)
 {
     const unsigned vecs = (g.hidden + Vec<DT>::N - 1) / Vec<DT>::N;
-#define QUANT(L, V) k_quant_rows<DT, L, V><<<dim3(L <= 64 ? (g.rows + ROWS(L) - 1) / ROWS(L) : g.rows), L <= 64 ? 256 : L, 0, st>>>(g)
+#define QUANT(L, V) k_quant_rows<DT, L, V><<<flat_grid(L <= 64 ? ((size_t)g.rows + ROWS(L) - 1) / ROWS(L) : g.rows), L <= 64 ? 256 : L, 0, st>>>(g)
 #define ROWS(L) (256 / (L <= 64 ? L : 64))
     if (vecs <= 8) QUANT(8, 1);
     else if (vecs <= 16) QUANT(16, 1);
@@ -195,7 +198,7 @@ template <int DT> void launch_quant(const RowsArgs& g, hipStream_t st)
     else if (vecs <= 1024) QUANT(256, 4);
     else if (vecs <= 2048) QUANT(512, 4);
     else if (vecs <= 4096) QUANT(1024, 4);
-    else k_quant_long<DT><<<dim3(g.rows), 1024, 0, st>>>(g);
+    else k_quant_long<DT><<<flat_grid(g.rows), 1024, 0, st>>>(g);
 #undef QUANT
 #undef ROWS
 }

@@ -10,6 +10,7 @@
 
 #include "../../include/tbvcoll.h"
 #include "tbv_device.h"
+#include "tbv_step.h"
 
 namespace tbv {
 
@@ -94,14 +95,18 @@ template <> struct Out<2> { typedef __bf16 T; [[maybe_unused]] static constexpr 
 
 // Which tile a block works on.  Blocks go to the eight XCDs in turn; each XCD gets a run of neighbouring tiles (bands of
 // `band` tile rows, column by column), so that the tiles its L2 serves at one time share rows of x and w.
-[[maybe_unused]] __device__ __forceinline__ void tile_of(unsigned b, unsigned tiles_m, unsigned tiles_n, unsigned band, unsigned* tm, unsigned* tn)
+[[maybe_unused]] __device__ __forceinline__ bool tile_of(unsigned tiles_m, unsigned tiles_n, unsigned band, unsigned* tm, unsigned* tn)
 {
-    const unsigned total = tiles_m * tiles_n, xcd = b & 7, q = total >> 3, r = total & 7;
+    const size_t block = flat_block();
+    const unsigned total = tiles_m * tiles_n, b = (unsigned)block;
+    if (block >= total) return false;                 // the rest of a grid's last row
+    const unsigned xcd = b & 7, q = total >> 3, r = total & 7;
     const unsigned p = (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + (b >> 3);
     const unsigned per_band = band * tiles_n, first = p / per_band * band, in = p % per_band;
     const unsigned rows = tiles_m - first < band ? tiles_m - first : band;
     *tm = first + in % rows;
     *tn = in / rows;
+    return true;
 }
 
 template <int DT, int TM, int TN, int S, int G>
@@ -115,7 +120,7 @@ __global__ __launch_bounds__(256 * G, TM * TN >= 8 ? 1 : 2) void k_mat_tile(MatA
     __shared__ __attribute__((aligned(1024))) signed char smem[G * STAGES];
     const unsigned tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6 & 3), group = __builtin_amdgcn_readfirstlane(tid >> 8);
     unsigned tm, tn;
-    tile_of(blockIdx.x, (g.m + BM - 1) / BM, (g.n + BN - 1) / BN, TM >= 4 ? 4 : 8, &tm, &tn);
+    if (!tile_of((g.m + BM - 1) / BM, (g.n + BN - 1) / BN, TM >= 4 ? 4 : 8, &tm, &tn)) return;
     const unsigned m0 = __builtin_amdgcn_readfirstlane(tm * BM), n0 = __builtin_amdgcn_readfirstlane(tn * BN);
 
     // the tile's rows of either operand, as a buffer of its own: the offsets of a tile fit 32 bits
@@ -346,7 +351,7 @@ __global__ __launch_bounds__(256 * G, TM * TN >= 8 ? 1 : 2) void k_mat_tile(MatA
 template <int DT, int TM, int TN, int S, int G> void launch_tile(const MatArgs& g, hipStream_t st)
 {
     const size_t tiles = (size_t)((g.m + 64 * TM - 1) / (64 * TM)) * ((g.n + 64 * TN - 1) / (64 * TN));
-    k_mat_tile<DT, TM, TN, S, G><<<dim3((unsigned)tiles), 256 * G, 0, st>>>(g);
+    k_mat_tile<DT, TM, TN, S, G><<<flat_grid(tiles), 256 * G, 0, st>>>(g);
 }
 
 // ------------------------------------------------------------------ few rows of x: the weights' bytes are the work
@@ -492,7 +497,7 @@ __global__ __launch_bounds__(256, 2) void k_mat_any(MatArgs g)
     __shared__ __attribute__((aligned(1024))) signed char sx[2][128 * 128], sw[2][128 * 128];
     const unsigned tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     unsigned tm, tn;
-    tile_of(blockIdx.x, (g.m + 127) / 128, (g.n + 127) / 128, 8, &tm, &tn);
+    if (!tile_of((g.m + 127) / 128, (g.n + 127) / 128, 8, &tm, &tn)) return;
     const unsigned m0 = tm * 128, n0 = tn * 128, at = ((lane & 7) ^ (lane >> 4) ^ (wave & 1) << 2) * 16;
     const signed char *xr[4], *wr[4];
 #pragma unroll
@@ -580,7 +585,7 @@ __global__ __launch_bounds__(256, 2) void k_mat_any(MatArgs g)
 template <int DT> void launch_any(const MatArgs& g, hipStream_t st)
 {
     const size_t tiles = (size_t)((g.m + 127) / 128) * ((g.n + 127) / 128);
-    k_mat_any<DT><<<dim3((unsigned)tiles), 256, 0, st>>>(g);
+    k_mat_any<DT><<<flat_grid(tiles), 256, 0, st>>>(g);
 }
 
 // The kernels a product of whole 16-byte pieces can take, as tiles: rows of x by rows of w.  What a tile costs on a CU by
@@ -609,7 +614,7 @@ template <int N> int pick_tile(const Tile (&tiles)[N], unsigned m, unsigned n, u
     for (int i = 0; i < N; i++) {
         const Tile& t = tiles[i];
         const size_t tm = ((size_t)m + t.rows - 1) / t.rows, tn = ((size_t)n + t.cols - 1) / t.cols;
-        if (t.ring && tm > 65535) continue;           // a grid's y
+        if (t.ring && (tm > 65535 || tn > (1u << 20))) continue;      // a grid's y and x
         const float us = (float)((tm * tn + 255) / 256) * (t.end + steps * t.step);
         if (least == 0.0f || us < least) { best = i; least = us; }
     }
@@ -661,7 +666,7 @@ inline bool meet(const void* p, size_t pn, const void* q, size_t qn)
 {
     return p && q && pn && qn && (uintptr_t)p < (uintptr_t)q + qn && (uintptr_t)q < (uintptr_t)p + pn;
 }
-inline size_t extent(size_t rows, size_t stride, size_t cols) { return rows && cols ? (rows - 1) * stride + cols : 0; }
+inline size_t extent(size_t rows, size_t stride, size_t cols) { return !rows || !cols ? 0 : rows > 1 ? (rows - 1) * stride + cols : cols; }
 }  // namespace
 
 extern "C" int tbv_step_matmul_i8(const tbv_matmul_i8* c, void* stream)
@@ -687,7 +692,8 @@ extern "C" int tbv_step_matmul_i8(const tbv_matmul_i8* c, void* stream)
         meet(c->out, out_bytes, c->bias, (size_t)c->n * esz)) MAT_FAIL("out overlaps an operand");
     MatArgs g{};
     g.out = c->out; g.x = c->x; g.x_scale = c->x_scale; g.w = c->w; g.w_scale = c->w_scale; g.bias = c->bias;
-    g.out_stride = (size_t)c->out_stride; g.x_stride = (size_t)c->x_stride; g.w_stride = (size_t)c->w_stride;
+    // (a single row has no stride, whatever was given)
+    g.out_stride = c->m > 1 ? (size_t)c->out_stride : 0; g.x_stride = c->m > 1 ? (size_t)c->x_stride : 0; g.w_stride = c->n > 1 ? (size_t)c->w_stride : 0;
     g.m = (unsigned)c->m; g.n = (unsigned)c->n; g.k = (unsigned)c->k;
     g.x_scale_step = c->x_scales != 1; g.w_scale_step = c->w_scales != 1;
     hipStream_t st = (hipStream_t)stream;

@@ -16,6 +16,7 @@
 
 #include "../../include/tbvcoll.h"
 #include "tbv_device.h"
+#include "tbv_step.h"
 
 namespace tbv {
 
@@ -72,9 +73,10 @@ __device__ __forceinline__ void turn_table(const RotArgs& g, unsigned total, flo
 {
     const unsigned tid = (threadIdx.z * blockDim.y + threadIdx.y) * blockDim.x + threadIdx.x, threads = blockDim.x * blockDim.y * blockDim.z;
     for (unsigned e = tid; e < g.half * blockDim.z; e += threads) {
-        const unsigned z = e / g.half, r = blockIdx.x * blockDim.z + z;
+        const unsigned z = e / g.half;
+        const size_t r = flat_block() * blockDim.z + z;
         float c, s;
-        if (r < total) { turn(g, r / g.tokens, r % g.tokens, e - z * g.half, &c, &s); table[e] = make_float2(c, s); }
+        if (r < total) { turn(g, (unsigned)r / g.tokens, (unsigned)r % g.tokens, e - z * g.half, &c, &s); table[e] = make_float2(c, s); }
     }
     __syncthreads();
 }
@@ -130,8 +132,8 @@ __global__ __launch_bounds__(512) void k_rotary(RotArgs g, unsigned total)
     constexpr unsigned N = Lanes<DT>::N, P = INTER ? N / 2 : N;          // elements and pairs of a unit
     constexpr ptrdiff_t ESZ = 16 / N;
     extern __shared__ float2 turns[];                 // [z][half]
-    const unsigned row = blockIdx.x * blockDim.z + threadIdx.z;           // batch and token
-    const unsigned token = row % g.tokens, batch = row / g.tokens;
+    const size_t row = flat_block() * blockDim.z + threadIdx.z;           // batch and token
+    const unsigned token = (unsigned)row % g.tokens, batch = (unsigned)row / g.tokens;
     // what a head is made of: whole units of pairs, single pairs, whole vectors to copy, single elements to copy
     const unsigned full = g.half / P, rest = g.head - 2 * g.half, pairs = full + g.half % P, vecs = pairs + rest / N, slots = vecs + rest % N;
     const unsigned heads = g.h[0].heads + g.h[1].heads, apart = g.half * ESZ;   // bytes between the halves
@@ -239,7 +241,7 @@ template <int DT> void launch_rot(const RotArgs& g, bool inter, unsigned total, 
     unsigned z = 256 / (x * y);
     while (z > 1 && (total / z < 1024 || g.half * z > kRotPairs)) z--;
     if (z < 1) z = 1;
-    const dim3 grid((total + z - 1) / z), block(x, y, z);
+    const dim3 grid = flat_grid(((size_t)total + z - 1) / z), block(x, y, z);
     const size_t lds = (size_t)g.half * z * sizeof(float2);
 #define ROT(I, U) k_rotary<DT, I, U><<<grid, block, lds, st>>>(g, total)
     if (inter) { if (per == 4) ROT(true, 4); else if (per == 2) ROT(true, 2); else ROT(true, 1); }

@@ -482,7 +482,7 @@ def linear_int8_all_reduce(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tens
     initialised, over the cap): the caller then runs its own layer."""
     _need(x.is_cuda and x.dim() >= 1 and w.dim() == 2, "x has to be on the GPU and w a matrix")
     n = w.shape[0]
-    if _lib is None or x.numel() // max(1, x.shape[-1]) * n * x.element_size() > _cap:
+    if _lib is None or math.prod(x.shape[:-1]) * n * x.element_size() > _cap:
         return None
     _need(out is None or (out.dtype is x.dtype and out.is_contiguous()), "out has to be contiguous and of x's type")
     codes, scale = quantize_int8(x)

@@ -507,6 +507,50 @@ def test_rotary_inverse_is_the_gradient(interleaved):
 
 
 @gpu
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_in_an_autograd_function(interleaved):
+    """The backward pass as a training program has it, a shared (expanded) key head among the inputs, against autograd
+    through the plain formula in 64 bits on the CPU; captured into a graph with leaves of its own."""
+    t, hq, hk, d, scale = 5, 4, 2, 32, 1.25
+    pos = torch.tensor([0, 7, 70000, 3, 3], device="cuda")
+    freqs, _ = tbvcoll.rotary_frequencies(24)
+
+    class Rotary(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, q, k):
+            return tbvcoll.rotary(q, k, pos, freqs, scale=scale, interleaved=interleaved, q_out=torch.empty_like(q), k_out=k.new_empty(k.shape))
+
+        @staticmethod
+        def backward(ctx, gq, gk):
+            return tbvcoll.rotary(gq, gk, pos, freqs, scale=scale, interleaved=interleaved, inverse=True, q_out=gq.new_empty(gq.shape), k_out=gk.new_empty(gk.shape))
+
+    q, k = (dev(synth.normal(i, t * h * d), torch.float32).view(t, h, d) for i, h in ((1, hq), (2, 1)))
+    gq, gk = (dev(synth.normal(i, t * h * d), torch.float32).view(t, h, d) for i, h in ((3, hq), (4, hk)))
+    q.requires_grad_(), k.requires_grad_()
+
+    def grads():
+        yq, yk = Rotary.apply(q, k.expand(t, hk, d))
+        return torch.autograd.grad((yq, yk), (q, k), (gq, gk), retain_graph=True)
+
+    eager = grads()
+    wq, tq = want_rotary(gq[None], pos[None], freqs, scale, interleaved, True)
+    wk, tk = want_rotary(gk[None], pos[None], freqs, scale, interleaved, True)
+    check(eager[0], wq[0], tq[0], torch.float32, "dq")
+    # the shared head's gradient is the sum over its heads: one more rounding of each of the hk - 1 additions
+    check(eager[1], wk[0].sum(1, keepdim=True), tk[0].sum(1, keepdim=True) + U * wk[0].abs().sum(1, keepdim=True), torch.float32, "dk")
+    q2, k2 = q.detach().clone().requires_grad_(), k.detach().clone().requires_grad_()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = Rotary.apply(q2, k2.expand(t, hk, d))
+        caught = torch.autograd.grad(out, (q2, k2), (gq, gk))
+    for _ in range(3):
+        gq.mul_(1)                                                        # the program's own work between replays
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(caught[0], eager[0]) and torch.equal(caught[1], eager[1])
+
+
+@gpu
 def test_rotary_refusals():
     q, k = torch.zeros(4, 3, 64, device="cuda"), torch.zeros(4, 1, 64, device="cuda")
     pos, freqs = torch.arange(4, device="cuda"), torch.ones(32, dtype=torch.float64, device="cuda")
@@ -688,6 +732,36 @@ def test_first_calls_inside_a_capture():
     p = subprocess.run([sys.executable, "-c", FIRST_CALL_IN_A_CAPTURE.format(root=ROOT)], capture_output=True, text=True, timeout=240)
     for k in range(3):
         assert f"REPLAY {k} True" in p.stdout, (p.stdout, p.stderr[-2000:])
+
+
+@gpu
+@pytest.mark.parametrize("m,n,k", [(1 << 21, 16, 16), (1100000, 3, 5), (2, (1 << 24) + 17, 16), (70000, 40, 33)])
+def test_product_of_very_many_rows(m, n, k):
+    """Rows beyond a grid's y, columns beyond its x: every result against the definition in int64."""
+    x, w = codes_of(1, 4096, k).cuda().repeat((m + 4095) // 4096, 1)[:m], codes_of(2, 4096, k).cuda().repeat((n + 4095) // 4096, 1)[:n]
+    one = torch.ones(1, device="cuda")
+    say("product", m, n, k)
+    got = tbvcoll.matmul_int8(x, one, w, one, dtype=torch.float32)
+    if m > n:
+        want = torch.matmul(x.float(), w.float().t().contiguous())              # below 2^24: exact in fp32
+    else:
+        want = torch.matmul(w.float(), x.float().t().contiguous()).t()
+    assert torch.equal(got, want)
+
+
+@gpu
+def test_more_threads_than_a_launch_dimension_holds():
+    """16.9 million rows of a block each: 2^32 threads and more in one launch."""
+    rows, cols = 16_900_000, 1025
+    x = torch.zeros(rows, cols, dtype=torch.bfloat16, device="cuda")
+    tail = dev(synth.normal(4, 3 * cols), torch.bfloat16).view(3, cols)
+    x[-3:] = tail
+    x[1 << 20] = tail[0]
+    say("quantize", rows, cols)
+    codes, scale = tbvcoll.quantize_int8(x)
+    c, s = want_rows(tail)
+    assert torch.equal(codes[-3:].cpu(), c) and torch.equal(scale[-3:].cpu(), s)
+    assert torch.equal(codes[1 << 20].cpu(), c[0]) and int((scale != 2.0 ** -126).sum()) == 4
 
 
 @gpu
