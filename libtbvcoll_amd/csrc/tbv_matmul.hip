@@ -247,7 +247,8 @@ __global__ __launch_bounds__(256 * G, TM * TN >= 8 ? 1 : 2) void k_mat_tile(MatA
     }
 
     // Results leave by strips of 32 rows of x through the wave's own part of the LDS: a lane holds sixteen neighbouring
-    // columns of a row in each block, the strip is stored in whole rows of the wave's columns.
+    // columns of a row in each block, the strip is stored in whole rows of the wave's columns, non-temporally (8192 x 8192 x
+    // 4096 bf16 224 -> 218 us: the L2 is left to x and w).
     typedef typename Out<DT>::T T;
     constexpr int EPV = 16 / ESZ, VPR = 32 * TN * ESZ / 16;     // elements in 16 bytes, 16-byte vectors in a strip's row
     typedef T TV __attribute__((ext_vector_type(EPV)));
@@ -325,14 +326,14 @@ __global__ __launch_bounds__(256 * G, TM * TN >= 8 ? 1 : 2) void k_mat_tile(MatA
 #pragma unroll
             for (int u = 0; u < VPR / 2; u++) {
                 const unsigned v = u * 64 + lane, row = v / VPR, col = v % VPR * EPV;
-                *(u32x4*)(o + row * g.out_stride + col) = *(const u32x4*)(strip + row * PITCH + col * ESZ);
+                __builtin_nontemporal_store(*(const u32x4*)(strip + row * PITCH + col * ESZ), (u32x4*)(o + row * g.out_stride + col));
             }
         } else if (aligned) {                         // the last tiles: whole vectors up to the edge
 #pragma unroll 2
             for (int u = 0; u < VPR / 2; u++) {
                 const unsigned v = u * 64 + lane, row = v / VPR, col = v % VPR * EPV;
                 if (ms + row >= g.m) continue;
-                if (col + EPV <= cols) *(u32x4*)(o + row * g.out_stride + col) = *(const u32x4*)(strip + row * PITCH + col * ESZ);
+                if (col + EPV <= cols) __builtin_nontemporal_store(*(const u32x4*)(strip + row * PITCH + col * ESZ), (u32x4*)(o + row * g.out_stride + col));
                 else for (unsigned e = col; e < cols; e++) o[row * g.out_stride + e] = *(const T*)(strip + row * PITCH + e * ESZ);
             }
         } else {                                      // rows that do not start on 16 bytes: an element a lane

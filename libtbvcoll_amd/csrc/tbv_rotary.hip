@@ -124,7 +124,11 @@ template <> struct Lanes<0> {
 };
 
 __device__ __forceinline__ u32x4 load16(const char* p) { u32x4 v; __builtin_memcpy(&v, p, 16); return v; }
-__device__ __forceinline__ void store16(char* p, u32x4 v) { __builtin_memcpy(p, &v, 16); }
+// (non-temporal: a result that stays in the L2 until the kernel ends stands between it and the next one; 2048 tokens of
+// 40 heads of 128 bf16 12.0 -> 8.3 us, 8191 of 20 heads fp16 20.7 -> 18.8.  Non-temporal loads gain 3 % more at best and
+// lose 40 % where heads do not start on 16 bytes.)
+typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
+__device__ __forceinline__ void store16(char* p, u32x4 v) { __builtin_nontemporal_store((u32x4_any)v, (u32x4_any*)p); }
 
 template <int DT, bool INTER, int U>
 __global__ __launch_bounds__(512) void k_rotary(RotArgs g, unsigned total)
