@@ -112,16 +112,9 @@ template <int DT> __device__ __forceinline__ void store_codes(signed char* row, 
         const uint32_t lo = __builtin_amdgcn_perm(t[4 * e + 1], t[4 * e], 0x0c0c0400u), hi = __builtin_amdgcn_perm(t[4 * e + 3], t[4 * e + 2], 0x04000c0cu);
         o[e] = fine ? lo | hi : 0u;
     }
-    // (non-temporal: codes that stay in the L2 until the kernel ends stand between it and the next one; 2048 x 4096 bf16
-    // 8.2 -> 6.6 us.  Non-temporal loads of x too: 6.8 there, 18.6 instead of 19.5 at 8192 x 4096: not done, since x has
-    // mostly just been written.)
-    typedef uint32_t Codes __attribute__((ext_vector_type(N / 4), aligned(1)));
-    if ((j + 1) * N <= hidden) {
-        Codes c;
-#pragma unroll
-        for (int e = 0; e < N / 4; e++) c[e] = o[e];
-        __builtin_nontemporal_store(c, (Codes*)(row + (size_t)j * N));
-    }
+    // (Ordinary stores: non-temporal ones make the kernel itself faster, 8.2 -> 6.6 us at 2048 x 4096 bf16, but the product
+    // that reads the codes next then finds them in no cache: with a multiply by the scales behind it 30.5 -> 33.4 us.)
+    if ((j + 1) * N <= hidden) __builtin_memcpy(row + (size_t)j * N, o, N);
     else for (unsigned e = 0; j * N + e < hidden; e++) row[(size_t)j * N + e] = (signed char)(o[e >> 2] >> (8 * (e & 3)));
 }
 

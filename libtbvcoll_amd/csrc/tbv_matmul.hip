@@ -27,6 +27,7 @@ struct MatArgs {
     size_t out_stride, x_stride, w_stride;
     unsigned m, n, k;
     unsigned x_scale_step, w_scale_step;      // 1, or 0 for one scale of the whole operand
+    int through;                              // store non-temporally
 };
 
 template <int DT> __device__ __forceinline__ float mat_elem(const void* p, size_t i)
@@ -247,8 +248,7 @@ __global__ __launch_bounds__(256 * G, TM * TN >= 8 ? 1 : 2) void k_mat_tile(MatA
     }
 
     // Results leave by strips of 32 rows of x through the wave's own part of the LDS: a lane holds sixteen neighbouring
-    // columns of a row in each block, the strip is stored in whole rows of the wave's columns, non-temporally (8192 x 8192 x
-    // 4096 bf16 224 -> 218 us: the L2 is left to x and w).
+    // columns of a row in each block, the strip is stored in whole rows of the wave's columns.
     typedef typename Out<DT>::T T;
     constexpr int EPV = 16 / ESZ, VPR = 32 * TN * ESZ / 16;     // elements in 16 bytes, 16-byte vectors in a strip's row
     typedef T TV __attribute__((ext_vector_type(EPV)));
@@ -323,17 +323,21 @@ __global__ __launch_bounds__(256 * G, TM * TN >= 8 ? 1 : 2) void k_mat_tile(MatA
         __builtin_amdgcn_wave_barrier();
         T* const o = (T*)g.out + (size_t)ms * g.out_stride + nw;
         if (whole && ms + 32 <= g.m) {
+            const auto rows = [&](auto store) {
 #pragma unroll
-            for (int u = 0; u < VPR / 2; u++) {
-                const unsigned v = u * 64 + lane, row = v / VPR, col = v % VPR * EPV;
-                __builtin_nontemporal_store(*(const u32x4*)(strip + row * PITCH + col * ESZ), (u32x4*)(o + row * g.out_stride + col));
-            }
+                for (int u = 0; u < VPR / 2; u++) {
+                    const unsigned v = u * 64 + lane, row = v / VPR, col = v % VPR * EPV;
+                    store(*(const u32x4*)(strip + row * PITCH + col * ESZ), (u32x4*)(o + row * g.out_stride + col));
+                }
+            };
+            if (g.through) rows([](u32x4 v, u32x4* p) { __builtin_nontemporal_store(v, p); });
+            else rows([](u32x4 v, u32x4* p) { *p = v; });
         } else if (aligned) {                         // the last tiles: whole vectors up to the edge
 #pragma unroll 2
             for (int u = 0; u < VPR / 2; u++) {
                 const unsigned v = u * 64 + lane, row = v / VPR, col = v % VPR * EPV;
                 if (ms + row >= g.m) continue;
-                if (col + EPV <= cols) __builtin_nontemporal_store(*(const u32x4*)(strip + row * PITCH + col * ESZ), (u32x4*)(o + row * g.out_stride + col));
+                if (col + EPV <= cols) *(u32x4*)(o + row * g.out_stride + col) = *(const u32x4*)(strip + row * PITCH + col * ESZ);
                 else for (unsigned e = col; e < cols; e++) o[row * g.out_stride + e] = *(const T*)(strip + row * PITCH + e * ESZ);
             }
         } else {                                      // rows that do not start on 16 bytes: an element a lane
@@ -697,6 +701,9 @@ extern "C" int tbv_step_matmul_i8(const tbv_matmul_i8* c, void* stream)
     g.out_stride = c->m > 1 ? (size_t)c->out_stride : 0; g.x_stride = c->m > 1 ? (size_t)c->x_stride : 0; g.w_stride = c->n > 1 ? (size_t)c->w_stride : 0;
     g.m = (unsigned)c->m; g.n = (unsigned)c->n; g.k = (unsigned)c->k;
     g.x_scale_step = c->x_scales != 1; g.w_scale_step = c->w_scales != 1;
+    // A result that the caches do not hold until it is read leaves them to x and w; with a copy of the result behind the
+    // product, 134 MB (8192 x 8192 bf16): 276 -> 270 us, but 34 MB (2048 x 8192): 69 -> 72.
+    g.through = out_bytes >= ((size_t)64 << 20);
     hipStream_t st = (hipStream_t)stream;
     switch (c->dtype) {
         case 0: launch_mat<0>(g, st); break;

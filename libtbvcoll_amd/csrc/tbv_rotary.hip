@@ -34,6 +34,7 @@ struct RotArgs {
     unsigned tokens, head, half, pos64;
     float scale;
     int inverse;
+    int through;                                // store non-temporally
 };
 
 template <int DT> __device__ __forceinline__ float rot_load(const void* p, ptrdiff_t i)
@@ -124,11 +125,12 @@ template <> struct Lanes<0> {
 };
 
 __device__ __forceinline__ u32x4 load16(const char* p) { u32x4 v; __builtin_memcpy(&v, p, 16); return v; }
-// (non-temporal: a result that stays in the L2 until the kernel ends stands between it and the next one; 2048 tokens of
-// 40 heads of 128 bf16 12.0 -> 8.3 us, 8191 of 20 heads fp16 20.7 -> 18.8.  Non-temporal loads gain 3 % more at best and
-// lose 40 % where heads do not start on 16 bytes.)
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
-__device__ __forceinline__ void store16(char* p, u32x4 v) { __builtin_nontemporal_store((u32x4_any)v, (u32x4_any*)p); }
+__device__ __forceinline__ void store16(char* p, u32x4 v, int through)
+{
+    if (through) __builtin_nontemporal_store((u32x4_any)v, (u32x4_any*)p);
+    else __builtin_memcpy(p, &v, 16);
+}
 
 template <int DT, bool INTER, int U>
 __global__ __launch_bounds__(512) void k_rotary(RotArgs g, unsigned total)
@@ -191,7 +193,7 @@ __global__ __launch_bounds__(512) void k_rotary(RotArgs g, unsigned total)
                             p[2 * e] = x[2 * e] * w[e].x - x[2 * e + 1] * w[e].y;
                             p[2 * e + 1] = x[2 * e + 1] * w[e].x + x[2 * e] * w[e].y;
                         }
-                        store16(out[u] + i * 16, Lanes<DT>::pack(p));
+                        store16(out[u] + i * 16, Lanes<DT>::pack(p), g.through);
                     } else {
                         Lanes<DT>::unpack(b[u], y);
 #pragma unroll
@@ -199,8 +201,8 @@ __global__ __launch_bounds__(512) void k_rotary(RotArgs g, unsigned total)
                             p[e] = x[e] * w[e].x - y[e] * w[e].y;
                             q[e] = y[e] * w[e].x + x[e] * w[e].y;
                         }
-                        store16(out[u] + i * 16, Lanes<DT>::pack(p));
-                        store16(out[u] + i * 16 + apart, Lanes<DT>::pack(q));
+                        store16(out[u] + i * 16, Lanes<DT>::pack(p), g.through);
+                        store16(out[u] + i * 16 + apart, Lanes<DT>::pack(q), g.through);
                     }
                 }
             } else if (i < pairs) {
@@ -219,7 +221,7 @@ __global__ __launch_bounds__(512) void k_rotary(RotArgs g, unsigned total)
 #pragma unroll
                 for (int u = 0; u < U; u++) {
                     if (u >= live || out[u] == in[u]) continue;
-                    if (i < vecs) store16(out[u] + (2 * g.half + (i - pairs) * N) * ESZ, a[u]);
+                    if (i < vecs) store16(out[u] + (2 * g.half + (i - pairs) * N) * ESZ, a[u], g.through);
                     else { const unsigned e = 2 * g.half + (rest / N) * N + i - vecs; rot_copy<DT>(out[u], e, in[u], e); }
                 }
             }
@@ -387,6 +389,11 @@ extern "C" int tbv_step_rotary(const tbv_rotary* c, void* stream)
     g.tokens = (unsigned)c->tokens; g.head = (unsigned)c->head; g.half = (unsigned)(c->rot / 2); g.pos64 = c->pos64 != 0;
     g.scale = c->scale; g.inverse = c->inverse != 0;
     const unsigned blocks = (unsigned)(c->batch * c->tokens);
+    // Results that fit the Infinity Cache but not the L2s are written past these: what is still there when the kernel ends
+    // stands between it and the next one.  Alone, and with a copy of the result behind it: 21 MB (2048 tokens of 40 heads of
+    // 128 bf16) 11.7 -> 8.7 and 18.2 -> 17.7 us; 5 MB 5.6 -> 5.0 and 8.4 -> 8.7; 84 MB 35.8 -> 35.5 and 63.5 -> 65.1.
+    const size_t result = (size_t)blocks * (size_t)(c->q.heads + c->k.heads) * (size_t)c->head * esz;
+    g.through = result >= ((size_t)16 << 20) && result <= ((size_t)64 << 20);
     hipStream_t st = (hipStream_t)stream;
     switch (c->dtype) {
         case 0: launch_rot<0>(g, c->interleaved != 0, blocks, st); break;
