@@ -27,7 +27,6 @@ struct MatArgs {
     size_t out_stride, x_stride, w_stride;
     unsigned m, n, k;
     unsigned x_scale_step, w_scale_step;      // 1, or 0 for one scale of the whole operand
-    int through;                              // store non-temporally
 };
 
 template <int DT> __device__ __forceinline__ float mat_elem(const void* p, size_t i)
@@ -110,7 +109,7 @@ template <> struct Out<2> { typedef __bf16 T; [[maybe_unused]] static constexpr 
     return true;
 }
 
-template <int DT, int TM, int TN, int S, int G>
+template <int DT, int TM, int TN, int S, int G, bool THROUGH>
 __global__ __launch_bounds__(256 * G, TM * TN >= 8 ? 1 : 2) void k_mat_tile(MatArgs g)
 {
 #ifdef __HIP_DEVICE_COMPILE__          // (register constraints and buffer loads the host pass does not know)
@@ -323,15 +322,14 @@ __global__ __launch_bounds__(256 * G, TM * TN >= 8 ? 1 : 2) void k_mat_tile(MatA
         __builtin_amdgcn_wave_barrier();
         T* const o = (T*)g.out + (size_t)ms * g.out_stride + nw;
         if (whole && ms + 32 <= g.m) {
-            const auto rows = [&](auto store) {
 #pragma unroll
-                for (int u = 0; u < VPR / 2; u++) {
-                    const unsigned v = u * 64 + lane, row = v / VPR, col = v % VPR * EPV;
-                    store(*(const u32x4*)(strip + row * PITCH + col * ESZ), (u32x4*)(o + row * g.out_stride + col));
-                }
-            };
-            if (g.through) rows([](u32x4 v, u32x4* p) { __builtin_nontemporal_store(v, p); });
-            else rows([](u32x4 v, u32x4* p) { *p = v; });
+            for (int u = 0; u < VPR / 2; u++) {
+                const unsigned v = u * 64 + lane, row = v / VPR, col = v % VPR * EPV;
+                const u32x4 d = *(const u32x4*)(strip + row * PITCH + col * ESZ);
+                u32x4* const to = (u32x4*)(o + row * g.out_stride + col);
+                if (THROUGH) __builtin_nontemporal_store(d, to);
+                else *to = d;
+            }
         } else if (aligned) {                         // the last tiles: whole vectors up to the edge
 #pragma unroll 2
             for (int u = 0; u < VPR / 2; u++) {
@@ -353,10 +351,10 @@ __global__ __launch_bounds__(256 * G, TM * TN >= 8 ? 1 : 2) void k_mat_tile(MatA
 #endif
 }
 
-template <int DT, int TM, int TN, int S, int G> void launch_tile(const MatArgs& g, hipStream_t st)
+template <int DT, int TM, int TN, int S, int G, bool THROUGH = false> void launch_tile(const MatArgs& g, hipStream_t st)
 {
     const size_t tiles = (size_t)((g.m + 64 * TM - 1) / (64 * TM)) * ((g.n + 64 * TN - 1) / (64 * TN));
-    k_mat_tile<DT, TM, TN, S, G><<<flat_grid(tiles), 256 * G, 0, st>>>(g);
+    k_mat_tile<DT, TM, TN, S, G, THROUGH><<<flat_grid(tiles), 256 * G, 0, st>>>(g);
 }
 
 // ------------------------------------------------------------------ few rows of x: the weights' bytes are the work
@@ -655,8 +653,13 @@ template <int DT> void launch_mat(const MatArgs& g, hipStream_t st)
         case 6: return launch_tile<DT, 2, 1, 2, 2>(g, st);
         case 7: return launch_tile<DT, 2, 2, 2, 1>(g, st);
         case 8: return launch_tile<DT, 2, 4, 2, 1>(g, st);
-        default: return launch_tile<DT, 4, 4, 2, 1>(g, st);
+        default: break;
     }
+    // A result that the caches do not hold until it is read is stored past them, which leaves them to x and w.  Alone, and with
+    // a copy of the result behind the product: 134 MB (8192 x 8192 bf16, k = 4096) 230 -> 223 and 276 -> 270 us; 34 MB
+    // (2048 x 8192) 61 -> 59, but 69 -> 72.
+    if ((size_t)g.m * g.n * Out<DT>::SIZE >= ((size_t)64 << 20)) return launch_tile<DT, 4, 4, 2, 1, true>(g, st);
+    launch_tile<DT, 4, 4, 2, 1>(g, st);
 }
 
 }  // namespace
@@ -701,9 +704,6 @@ extern "C" int tbv_step_matmul_i8(const tbv_matmul_i8* c, void* stream)
     g.out_stride = c->m > 1 ? (size_t)c->out_stride : 0; g.x_stride = c->m > 1 ? (size_t)c->x_stride : 0; g.w_stride = c->n > 1 ? (size_t)c->w_stride : 0;
     g.m = (unsigned)c->m; g.n = (unsigned)c->n; g.k = (unsigned)c->k;
     g.x_scale_step = c->x_scales != 1; g.w_scale_step = c->w_scales != 1;
-    // A result that the caches do not hold until it is read leaves them to x and w; with a copy of the result behind the
-    // product, 134 MB (8192 x 8192 bf16): 276 -> 270 us, but 34 MB (2048 x 8192): 69 -> 72.
-    g.through = out_bytes >= ((size_t)64 << 20);
     hipStream_t st = (hipStream_t)stream;
     switch (c->dtype) {
         case 0: launch_mat<0>(g, st); break;

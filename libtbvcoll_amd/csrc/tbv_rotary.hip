@@ -34,7 +34,7 @@ struct RotArgs {
     unsigned tokens, head, half, pos64;
     float scale;
     int inverse;
-    int through;                                // store non-temporally
+    bool through;                               // store non-temporally
 };
 
 template <int DT> __device__ __forceinline__ float rot_load(const void* p, ptrdiff_t i)
@@ -126,13 +126,13 @@ template <> struct Lanes<0> {
 
 __device__ __forceinline__ u32x4 load16(const char* p) { u32x4 v; __builtin_memcpy(&v, p, 16); return v; }
 typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
-__device__ __forceinline__ void store16(char* p, u32x4 v, int through)
+template <bool THROUGH> __device__ __forceinline__ void store16(char* p, u32x4 v)
 {
-    if (through) __builtin_nontemporal_store((u32x4_any)v, (u32x4_any*)p);
+    if (THROUGH) __builtin_nontemporal_store((u32x4_any)v, (u32x4_any*)p);
     else __builtin_memcpy(p, &v, 16);
 }
 
-template <int DT, bool INTER, int U>
+template <int DT, bool INTER, int U, bool THROUGH>
 __global__ __launch_bounds__(512) void k_rotary(RotArgs g, unsigned total)
 {
     constexpr unsigned N = Lanes<DT>::N, P = INTER ? N / 2 : N;          // elements and pairs of a unit
@@ -193,7 +193,7 @@ __global__ __launch_bounds__(512) void k_rotary(RotArgs g, unsigned total)
                             p[2 * e] = x[2 * e] * w[e].x - x[2 * e + 1] * w[e].y;
                             p[2 * e + 1] = x[2 * e + 1] * w[e].x + x[2 * e] * w[e].y;
                         }
-                        store16(out[u] + i * 16, Lanes<DT>::pack(p), g.through);
+                        store16<THROUGH>(out[u] + i * 16, Lanes<DT>::pack(p));
                     } else {
                         Lanes<DT>::unpack(b[u], y);
 #pragma unroll
@@ -201,8 +201,8 @@ __global__ __launch_bounds__(512) void k_rotary(RotArgs g, unsigned total)
                             p[e] = x[e] * w[e].x - y[e] * w[e].y;
                             q[e] = y[e] * w[e].x + x[e] * w[e].y;
                         }
-                        store16(out[u] + i * 16, Lanes<DT>::pack(p), g.through);
-                        store16(out[u] + i * 16 + apart, Lanes<DT>::pack(q), g.through);
+                        store16<THROUGH>(out[u] + i * 16, Lanes<DT>::pack(p));
+                        store16<THROUGH>(out[u] + i * 16 + apart, Lanes<DT>::pack(q));
                     }
                 }
             } else if (i < pairs) {
@@ -221,7 +221,7 @@ __global__ __launch_bounds__(512) void k_rotary(RotArgs g, unsigned total)
 #pragma unroll
                 for (int u = 0; u < U; u++) {
                     if (u >= live || out[u] == in[u]) continue;
-                    if (i < vecs) store16(out[u] + (2 * g.half + (i - pairs) * N) * ESZ, a[u], g.through);
+                    if (i < vecs) store16<THROUGH>(out[u] + (2 * g.half + (i - pairs) * N) * ESZ, a[u]);
                     else { const unsigned e = 2 * g.half + (rest / N) * N + i - vecs; rot_copy<DT>(out[u], e, in[u], e); }
                 }
             }
@@ -249,7 +249,10 @@ template <int DT> void launch_rot(const RotArgs& g, bool inter, unsigned total, 
     if (z < 1) z = 1;
     const dim3 grid = flat_grid(((size_t)total + z - 1) / z), block(x, y, z);
     const size_t lds = (size_t)g.half * z * sizeof(float2);
-#define ROT(I, U) k_rotary<DT, I, U><<<grid, block, lds, st>>>(g, total)
+#define ROT(I, U) do { \
+        if (g.through) k_rotary<DT, I, U, true><<<grid, block, lds, st>>>(g, total); \
+        else k_rotary<DT, I, U, false><<<grid, block, lds, st>>>(g, total); \
+    } while (0)
     if (inter) { if (per == 4) ROT(true, 4); else if (per == 2) ROT(true, 2); else ROT(true, 1); }
     else { if (per == 4) ROT(false, 4); else if (per == 2) ROT(false, 2); else ROT(false, 1); }
 #undef ROT
