@@ -81,10 +81,14 @@ __global__ __launch_bounds__(256) void k_mat_short(MatArgs g)
 // Four waves, two by two, compute a tile of 64 TM rows of x by 64 TN rows of w; a wave holds TM x TN blocks of 32 x 32 sums.
 // A step takes 128 bytes of k, whole cache lines (two steps of 64 halve the rate of the loads).  The buffer loads write the
 // LDS directly (no registers, no address arithmetic): 128 bytes of a row are eight lanes, and the piece a lane fetches is
-// rotated by the row so that the eight rows that eight lanes of a fragment read lie in different banks.  Two buffers:
-// while step t is multiplied, step t + 1 arrives, and t + 2 is asked for as soon as the last fragment of t has been read,
-// in the middle of the step.  Fragments are read half a step ahead of the products that use them, so a step has one
-// barrier and no product waits for the LDS.
+// rotated by the row so that the lanes that read a fragment together find it in different banks.  The LDS holds S steps of w
+// and S + 1 of x: step t + S of x is asked for at the start of step t, into the buffer of t - 1, and of w in its middle, once
+// the last fragment of t has been read.  Fragments are read half a step ahead of the products that use them, so a step has
+// one barrier and no product waits for the LDS.  G groups of four waves take the steps in turn and join their sums in the LDS,
+// for products with fewer tiles than the GPU has CUs.
+// What bounds it (2048 x 8192 x 4096 bf16 61 us, 8192 x 8192 x 4096 223 us: 2.25 and 2.46 POP/s, the library's product alone
+// takes 68 and 245): the matrix units, busy 68 % of the cycles, at the clock that the power limit leaves (1.85 GHz; the same
+// product of zeros takes three quarters of the time).
 typedef __attribute__((address_space(3))) void lds_void;
 
 template <int N> struct Int { static constexpr int value = N; };
@@ -142,16 +146,16 @@ __global__ __launch_bounds__(256 * G, TM * TN >= 8 ? 1 : 2) void k_mat_tile(MatA
     signed char* const stage = smem + group * STAGES;
 
     // ask for a step's rows of x or w; pieces beyond k (all of a step beyond the last) lie out of the buffer's range and
-    // arrive as zeros
+    // arrive as zeros (the scalar offset stays within it: the range check subtracts it)
     const auto fetch_x = [&](unsigned t, unsigned buf) {
-        const unsigned k0 = (t * G + group) * 128;
-        const bool past = k0 + xpiece * 16 >= g.k;
+        const unsigned at = (t * G + group) * 128, k0 = at < g.k ? at : 0;
+        const bool past = at + xpiece * 16 >= g.k;
 #pragma unroll
         for (int j = 0; j < 2 * TM; j++) __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (lds_void*)(stage + buf * XS + (j * 4 + wave) * 1024), 16, past ? 0x80000000u : xo[j], k0, 0, 0);
     };
     const auto fetch_w = [&](unsigned t, unsigned buf) {
-        const unsigned k0 = (t * G + group) * 128;
-        const bool past = k0 + wpiece * 16 >= g.k;
+        const unsigned at = (t * G + group) * 128, k0 = at < g.k ? at : 0;
+        const bool past = at + wpiece * 16 >= g.k;
 #pragma unroll
         for (int j = 0; j < 2 * TN; j++) __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (lds_void*)(stage + (S + 1) * XS + buf * WS + (j * 4 + wave) * 1024), 16, past ? 0x80000000u : wo[j], k0, 0, 0);
     };
@@ -386,8 +390,8 @@ __global__ __launch_bounds__(64 * W) void k_mat_rows(MatArgs g)
     for (int i = 0; i < 2 * MB; i++) { const unsigned r = i * 8 + (lane >> 3); xr_row[i] = r < mrows ? r : mrows - 1; xo[i] = xr_row[i] * (unsigned)g.x_stride + at; }
     signed char* const ring = smem + wave * RING;
     const auto fetch = [&](unsigned piece, int u) {
-        const unsigned k0 = piece * 128;
-        const bool past = k0 + at >= g.k;                              // out of the buffer's range: zeros
+        const unsigned k0 = piece * 128 < g.k ? piece * 128 : 0;       // (within the buffer: the range check subtracts it)
+        const bool past = piece * 128 + at >= g.k;                     // out of the buffer's range: zeros
 #pragma unroll
         for (int j = 0; j < 2 * NB; j++) __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (lds_void*)(ring + u * SLOT + j * 1024), 16, past ? 0x80000000u : wo[j], k0, 0, 0);
 #pragma unroll

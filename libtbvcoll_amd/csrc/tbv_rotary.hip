@@ -377,6 +377,13 @@ extern "C" int tbv_step_rotary(const tbv_rotary* c, void* stream)
     if (!c->q.heads && !c->k.heads) return 0;
     if (c->rot && (!c->positions || !c->freqs)) ROT_FAIL("null positions or freqs");
     if (((uintptr_t)c->positions % (c->pos64 ? 8 : 4)) || ((uintptr_t)c->freqs % 8)) ROT_FAIL("positions and freqs must be aligned to their elements");
+    // The extents of positions and freqs, to hold the outputs off them.
+    const int64_t far = (int64_t)1 << 56;
+    if ((c->batch > 1 && (c->pos_batch > far / (c->batch - 1) || c->pos_batch < -far / (c->batch - 1))) ||
+        (c->tokens > 1 && (c->pos_token > far / (c->tokens - 1) || c->pos_token < -far / (c->tokens - 1)))) ROT_FAIL("position strides that reach beyond 2^56");
+    const Span pos = span_of(Grid{c->positions, {(ptrdiff_t)c->pos_batch, (ptrdiff_t)c->pos_token, 0}, {(size_t)c->batch, (size_t)c->tokens, 1}}, 1, c->pos64 ? 8 : 4);
+    const Span freqs{(uintptr_t)c->freqs, (uintptr_t)c->freqs + (size_t)c->rot * 4};
+    for (int i = 0; i < 2; i++) if (g.h[i].heads && c->rot && (meet(spans_out[i], pos) || meet(spans_out[i], freqs))) ROT_FAIL("an output overlaps positions or freqs");
     // An output that is not its input is held apart from both inputs.  The two outputs, and an output in place and the
     // other's input, may be views of one buffer (a packed projection): they must have no element in common.
     for (int i = 0; i < 2; i++) {

@@ -362,7 +362,7 @@ def all_reduce_rmsnorm(t: torch.Tensor, weight: torch.Tensor, eps: float, out: t
 # ------------------------------------------------------------------ the layer around the all-reduce (additive)
 #
 # These need no `init` and have nothing to fall back to: a call they cannot take raises ValueError.  They run on the
-# current stream of the tensors' device.  A decode step makes hundreds of these calls, each on the GPU for a few
+# current stream of the tensors' device and record no gradient.  A decode step makes hundreds of these calls, each on the GPU for a few
 # microseconds, so they look at every attribute once and hand the library one packed structure.
 
 _step_lib = None
@@ -394,6 +394,12 @@ def _launch(fn, device, call):
         raise RuntimeError(f"{fn.__name__} failed rc={rc}")
 
 
+def _frozen():
+    """A tensor that requires a gradient: the kernels record none, so the call is for code that asks for none."""
+    if torch.is_grad_enabled():
+        raise ValueError("records no gradient: call it under torch.no_grad(), or in the forward and backward of a torch.autograd.Function")
+
+
 def _rows(t, what):
     """(rows, columns, row stride) of a tensor as a matrix of contiguous rows; leading dimensions are taken together."""
     if t.dim() == 2:
@@ -417,6 +423,8 @@ def quantize_int8(x: torch.Tensor, codes: torch.Tensor = None, scale: torch.Tens
     code, dev, shape = _DT.get(x.dtype), x.get_device(), x.shape
     if code is None or dev < 0:
         raise ValueError("x has to be a fp32, fp16 or bf16 tensor on the GPU")
+    if x.requires_grad:
+        _frozen()
     rows, cols, xs = _rows(x, "x")
     if codes is None:
         codes = torch.empty_like(x, dtype=torch.int8) if x.is_contiguous() else x.new_empty(shape, dtype=torch.int8)
@@ -440,7 +448,7 @@ def matmul_int8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale
     out = dtype(float(sum) * x_scale * w_scale + bias), the sum exact in int32.  x_scale: fp32, one per row of x (any
     shape of that many elements) or a single one; w_scale: fp32, n or one; bias: n elements of the result's type.
     Returns `out` [..., n] (its type counts when given).  k up to 131071; fastest where k and the row strides are
-    multiples of 16 and the tensors 16-byte aligned.  There is no gradient: the weights are frozen codes."""
+    multiples of 16 and the tensors 16-byte aligned."""
     dev = x.get_device()
     if dev < 0 or x.dtype is not torch.int8 or w.dtype is not torch.int8 or w.get_device() != dev or w.dim() != 2:
         raise ValueError("x and w have to be int8 on one GPU, w a matrix")
@@ -448,6 +456,8 @@ def matmul_int8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale
     n, wk, ws = _rows(w, "w")
     if k != wk or k > 131071:
         raise ValueError(f"x has rows of {k} and w of {wk}: they have to be equal, and at most 131071 (beyond, the int32 sum can overflow)")
+    if x_scale.requires_grad or w_scale.requires_grad or (bias is not None and bias.requires_grad):
+        _frozen()
     sx, sw = x_scale.numel(), w_scale.numel()
     if x_scale.dtype is not torch.float32 or x_scale.get_device() != dev or not x_scale.is_contiguous() or (sx != m and sx != 1):
         raise ValueError("x_scale has to be contiguous fp32 on x's device, one for each row of x or one for all")
@@ -560,6 +570,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, freqs: tor
     d = len(shape)
     if dev < 0 or code is None or (d != 3 and d != 4):
         raise ValueError("q has to be fp32, fp16 or bf16 on the GPU, [tokens, heads, head] or [batch, tokens, heads, head]")
+    if q.requires_grad or (k is not None and k.requires_grad):
+        _frozen()
     batch, tokens, head = 1 if d == 3 else shape[0], shape[-3], shape[-1]
     if q_out is None:
         q_out = q

@@ -219,6 +219,13 @@ def test_refused_rotary_calls(q, k, kw, capfd):
     assert "[tbvcoll] rotary:" in capfd.readouterr().err
 
 
+@pytest.mark.parametrize("kw", [dict(positions=P), dict(positions=P + 8 * 256 * 4 - 8), dict(positions=3 * P - 8), dict(freqs=3 * P + 8), dict(freqs=P - 248),
+                                dict(positions=P + 16384, pos_batch=-8), dict(pos_token=1 << 55), dict(pos_batch=-(1 << 57))])
+def test_rotary_outputs_stay_off_positions_and_freqs(kw, capfd):
+    assert rot_call(**kw) == -1
+    assert "[tbvcoll] rotary:" in capfd.readouterr().err
+
+
 def test_empty_rotary_calls_launch_nothing():
     assert rot_call(batch=0) == 0 and rot_call(tokens=0) == 0 and rot_call(head=0, rot=0) == 0
     assert rot_call(dict(heads=0, out=0), dict(heads=0, out=0)) == 0
@@ -762,6 +769,40 @@ def test_more_threads_than_a_launch_dimension_holds():
     c, s = want_rows(tail)
     assert torch.equal(codes[-3:].cpu(), c) and torch.equal(scale[-3:].cpu(), s)
     assert torch.equal(codes[1 << 20].cpu(), c[0]) and int((scale != 2.0 ** -126).sum()) == 4
+
+
+@gpu
+@pytest.mark.parametrize("m,n", [(1, 1), (2, 1), (1, 3), (17, 1), (40, 2), (130, 1), (300, 300)])
+@pytest.mark.parametrize("k", [16, 32, 144])
+def test_product_of_a_few_bytes(m, n, k):
+    """Operands that end long before the loads that run ahead would: the buffers' range is what stops those."""
+    x, w = codes_of(1, m, k).cuda(), codes_of(2, n, k).cuda()
+    xs, ws = scales_of(3, m).cuda(), scales_of(4, n).cuda()
+    say("product", m, n, k)
+    got = tbvcoll.matmul_int8(x, xs, w, ws, dtype=torch.float32)
+    sums = x.cpu().long() @ w.cpu().long().t()
+    assert torch.equal(got.cpu(), sums.float() * xs.cpu()[:, None] * ws.cpu()[None])
+
+
+@gpu
+def test_tensors_that_ask_for_a_gradient_are_refused():
+    """The kernels record no gradient: silently dropping one is an error, unless nobody asked for it."""
+    x = torch.ones(4, 64, device="cuda", requires_grad=True)
+    codes, scale = torch.ones(4, 64, dtype=torch.int8, device="cuda"), torch.ones(4, device="cuda")
+    learned = torch.ones(4, device="cuda", requires_grad=True)
+    pos, freqs = torch.arange(4, device="cuda"), torch.ones(8, dtype=torch.float64, device="cuda")
+    calls = [lambda: tbvcoll.quantize_int8(x), lambda: tbvcoll.matmul_int8(codes, learned, codes, scale), lambda: tbvcoll.matmul_int8(codes, scale, codes, learned),
+             lambda: tbvcoll.matmul_int8(codes, scale, codes, scale, bias=learned, dtype=torch.float32),
+             lambda: tbvcoll.rotary(x.view(4, 4, 16), None, pos, freqs), lambda: tbvcoll.rotary(x.detach().clone().view(4, 4, 16), x.view(4, 4, 16), pos, freqs)]
+    for call in calls:
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+    assert bool((x == 1).all())
+    with torch.no_grad():
+        for call in calls:
+            call()
+    with torch.inference_mode():
+        calls[1]()
 
 
 @gpu
