@@ -371,6 +371,10 @@ _MATMUL = struct.Struct("6P9q")            # tbv_matmul_i8
 _ROTARY = struct.Struct("2P7q2P7q2P10qf4x")  # tbv_rotary
 
 
+_WIDE = {torch.int64: 1, torch.int32: 0}
+_NO_HEADS = (0,) * 9
+
+
 def _steps():
     global _step_lib
     if _step_lib is None:
@@ -400,16 +404,18 @@ def _frozen():
         raise ValueError("records no gradient: call it under torch.no_grad(), or in the forward and backward of a torch.autograd.Function")
 
 
-def _rows(t, what):
-    """(rows, columns, row stride) of a tensor as a matrix of contiguous rows; leading dimensions are taken together."""
-    if t.dim() == 2:
-        r, c = t.shape
+def _rows(t, shape, what):
+    """(rows, columns, row stride) of a tensor of this shape as a matrix of contiguous rows; leading dimensions are taken together."""
+    if len(shape) == 2:
+        r, c = shape
         s, e = t.stride()
+    elif shape:
+        c, e = shape[-1], t.stride(-1)
+        r, s = math.prod(shape[:-1]), c
+        if len(shape) > 1 and r * c and not t.is_contiguous():
+            raise ValueError(what + ": leading dimensions have to be contiguous")
     else:
-        _need(t.dim() >= 1, what + " needs at least one dimension")
-        c, e = t.shape[-1], t.stride(-1)
-        r, s = math.prod(t.shape[:-1]), c
-        _need(t.dim() == 1 or t.is_contiguous() or r * c == 0, what + ": leading dimensions have to be contiguous")
+        raise ValueError(what + " needs at least one dimension")
     if (e != 1 and c > 1) or (s < c and r > 1):
         raise ValueError(what + ": the last dimension has to be contiguous and rows must not overlap")
     return r, c, s if r > 1 else c
@@ -425,18 +431,18 @@ def quantize_int8(x: torch.Tensor, codes: torch.Tensor = None, scale: torch.Tens
         raise ValueError("x has to be a fp32, fp16 or bf16 tensor on the GPU")
     if x.requires_grad:
         _frozen()
-    rows, cols, xs = _rows(x, "x")
+    rows, cols, xs = _rows(x, shape, "x")
     if codes is None:
         codes = torch.empty_like(x, dtype=torch.int8) if x.is_contiguous() else x.new_empty(shape, dtype=torch.int8)
         cs = cols
     else:
-        _need(codes.dtype is torch.int8 and codes.shape == shape and codes.get_device() == dev, "codes has to be int8, of x's shape and device")
-        cs = _rows(codes, "codes")[2]
+        if codes.dtype is not torch.int8 or codes.shape != shape or codes.get_device() != dev:
+            raise ValueError("codes has to be int8, of x's shape and device")
+        cs = _rows(codes, shape, "codes")[2]
     if scale is None:
         scale = x.new_empty(shape[:-1], dtype=torch.float32)
-    else:
-        _need(scale.dtype is torch.float32 and scale.shape == shape[:-1] and scale.get_device() == dev and scale.is_contiguous(),
-              "scale has to be contiguous fp32, of x's shape without its last dimension, on its device")
+    elif scale.dtype is not torch.float32 or scale.shape != shape[:-1] or scale.get_device() != dev or not scale.is_contiguous():
+        raise ValueError("scale has to be contiguous fp32, of x's shape without its last dimension, on its device")
     if rows:
         _launch((_step_lib or _steps()).tbv_step_quantize_i8, dev, _QUANTIZE.pack(codes.data_ptr(), scale.data_ptr(), x.data_ptr(), cs, xs, rows, cols, code))
     return codes, scale
@@ -449,11 +455,11 @@ def matmul_int8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale
     shape of that many elements) or a single one; w_scale: fp32, n or one; bias: n elements of the result's type.
     Returns `out` [..., n] (its type counts when given).  k up to 131071; fastest where k and the row strides are
     multiples of 16 and the tensors 16-byte aligned."""
-    dev = x.get_device()
-    if dev < 0 or x.dtype is not torch.int8 or w.dtype is not torch.int8 or w.get_device() != dev or w.dim() != 2:
+    dev, shape, channels = x.get_device(), x.shape, w.shape
+    if dev < 0 or x.dtype is not torch.int8 or w.dtype is not torch.int8 or w.get_device() != dev or len(channels) != 2:
         raise ValueError("x and w have to be int8 on one GPU, w a matrix")
-    m, k, xs = _rows(x, "x")
-    n, wk, ws = _rows(w, "w")
+    m, k, xs = _rows(x, shape, "x")
+    n, wk, ws = _rows(w, channels, "w")
     if k != wk or k > 131071:
         raise ValueError(f"x has rows of {k} and w of {wk}: they have to be equal, and at most 131071 (beyond, the int32 sum can overflow)")
     if x_scale.requires_grad or w_scale.requires_grad or (bias is not None and bias.requires_grad):
@@ -465,19 +471,23 @@ def matmul_int8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale
         raise ValueError("w_scale has to be contiguous fp32 on x's device, one for each row of w or one for all")
     if out is None:
         code, os_ = _DT.get(dtype), n
-        _need(code is not None, "the result is fp32, fp16 or bf16")
-        out = x_scale.new_empty((m, n) if x.dim() == 2 else x.shape[:-1] + (n,), dtype=dtype)
+        if code is None:
+            raise ValueError("the result is fp32, fp16 or bf16")
+        out = x_scale.new_empty((m, n) if len(shape) == 2 else shape[:-1] + (n,), dtype=dtype)
     else:
         dtype = out.dtype
         code = _DT.get(dtype)
-        _need(code is not None, "the result is fp32, fp16 or bf16")
-        _need(out.get_device() == dev and out.shape == x.shape[:-1] + (n,), "out has to be on x's device, of x's shape with n columns")
-        os_ = _rows(out, "out")[2]
+        if code is None:
+            raise ValueError("the result is fp32, fp16 or bf16")
+        wide = shape[:-1] + (n,)
+        if out.get_device() != dev or out.shape != wide:
+            raise ValueError("out has to be on x's device, of x's shape with n columns")
+        os_ = _rows(out, wide, "out")[2]
     if bias is None:
         b = 0
     else:
-        _need(bias.dtype is dtype and bias.get_device() == dev and bias.is_contiguous() and bias.numel() == n,
-              "bias has to be n contiguous elements of the result's type on x's device")
+        if bias.dtype is not dtype or bias.get_device() != dev or not bias.is_contiguous() or bias.numel() != n:
+            raise ValueError("bias has to be n contiguous elements of the result's type on x's device")
         b = bias.data_ptr()
     if m and n:
         _launch((_step_lib or _steps()).tbv_step_matmul_i8, dev, _MATMUL.pack(
@@ -542,19 +552,21 @@ def rotary_frequencies(rot: int, base: float = 10000.0, factor: float = 1.0, met
     return freqs.to(device), scale
 
 
-def _heads(t, o, what):
+def _heads(t, shape, o, what):
     """The nine fields of tbv_rotary_heads for t ([tokens, heads, head] or [batch, tokens, heads, head]) turned into o."""
     s = t.stride()
-    if o is t:
+    if o is None or o is t:
+        at = to = t.data_ptr()
         u = s
     else:
-        _need(o.dtype is t.dtype and o.get_device() == t.get_device() and o.shape == t.shape, what + "_out has to be of its input's type, device and shape")
-        u = o.stride()
-    if (s[-1] != 1 or u[-1] != 1) and t.shape[-1] > 1:
+        if o.dtype is not t.dtype or o.get_device() != t.get_device() or o.shape != shape:
+            raise ValueError(what + "_out has to be of its input's type, device and shape")
+        u, at, to = o.stride(), t.data_ptr(), o.data_ptr()
+    if (s[-1] != 1 or u[-1] != 1) and shape[-1] > 1:
         raise ValueError(what + ": the elements of a head have to be contiguous")
     if len(s) == 3:
-        return o.data_ptr(), t.data_ptr(), t.shape[1], 0, s[0], s[1], 0, u[0], u[1]
-    return o.data_ptr(), t.data_ptr(), t.shape[2], s[0], s[1], s[2], u[0], u[1], u[2]
+        return to, at, shape[1], 0, s[0], s[1], 0, u[0], u[1]
+    return to, at, shape[2], s[0], s[1], s[2], u[0], u[1], u[2]
 
 
 def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, scale: float = 1.0,
@@ -573,33 +585,31 @@ def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, freqs: tor
     if q.requires_grad or (k is not None and k.requires_grad):
         _frozen()
     batch, tokens, head = 1 if d == 3 else shape[0], shape[-3], shape[-1]
-    if q_out is None:
-        q_out = q
-    hq = _heads(q, q_out, "q")
+    hq = _heads(q, shape, q_out, "q")
     if k is None:
-        _need(k_out is None, "k_out without k")
-        hk = (0,) * 9
+        if k_out is not None:
+            raise ValueError("k_out without k")
+        hk = _NO_HEADS
     else:
         ks = k.shape
-        if k.dtype is not q.dtype or k.get_device() != dev or len(ks) != d or ks[:-2] != shape[:-2] or ks[-1] != head:
+        if k.dtype is not q.dtype or k.get_device() != dev or len(ks) != d or ks[0] != shape[0] or ks[-3] != tokens or ks[-1] != head:
             raise ValueError("k has to be of q's type and device and differ in its heads only")
-        if k_out is None:
-            k_out = k
-        hk = _heads(k, k_out, "k")
-    pt, ps = positions.dtype, positions.shape
-    if positions.get_device() != dev or (pt is not torch.int64 and pt is not torch.int32):
+        hk = _heads(k, ks, k_out, "k")
+    wide, ps = _WIDE.get(positions.dtype), positions.shape
+    if positions.get_device() != dev or wide is None:
         raise ValueError("positions have to be int64 or int32 on q's device")
     if len(ps) == 1 and ps[0] == tokens:
-        p0, p1 = 0, positions.stride()[0]
-    else:
-        _need(d == 4 and ps == shape[:2], "positions have to be [tokens] or [batch, tokens]")
+        p0, p1 = 0, positions.stride(0)
+    elif d == 4 and ps == shape[:2]:
         p0, p1 = positions.stride()
+    else:
+        raise ValueError("positions have to be [tokens] or [batch, tokens]")
     rot = 2 * freqs.numel()
     if freqs.dtype is not torch.float64 or freqs.get_device() != dev or freqs.dim() != 1 or not freqs.is_contiguous() or rot > head or rot > 8192:
         raise ValueError("freqs has to be contiguous fp64 on q's device, at most half a head and 4096 long")
     _launch((_step_lib or _steps()).tbv_step_rotary, dev, _ROTARY.pack(
-        *hq, *hk, positions.data_ptr(), freqs.data_ptr(), p0, p1, batch, tokens, head, rot, code, pt is torch.int64, interleaved, inverse, scale))
-    return q_out, k_out
+        *hq, *hk, positions.data_ptr(), freqs.data_ptr(), p0, p1, batch, tokens, head, rot, code, wide, interleaved, inverse, scale))
+    return q if q_out is None else q_out, k if k_out is None else k_out
 
 
 def shutdown():
