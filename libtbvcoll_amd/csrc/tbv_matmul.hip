@@ -366,7 +366,11 @@ template <int DT, int TM, int TN, int S, int G, bool THROUGH = false> void launc
 // A block computes 16 NB columns for 16 MB rows of x; its W waves share out k in pieces of 128 bytes and their sums are
 // joined through the LDS (exact, so in any order).  Until then no wave waits for another: each has a ring of U pieces of
 // its own in the LDS, which the buffer loads fill in whole cache lines (fragments loaded straight into registers are 64
-// bytes of 16 rows a load, at half the rate: 7.1 against 6.1 us at 16 x 4096 x 4096).
+// bytes of 16 rows a load, at half the rate: 7.1 against 5.5 us at 16 x 4096 x 4096).  Blocks begin k at different pieces: rows
+// are often a power of two apart, and with all blocks at one column the loads meet in a few of the caches' and the memory's
+// channels (16 x 8192 x 4096 8.2 -> 7.1 us, 64 x 4096 x 8192 12.5 -> 8.7, 4 x 8192 x 8192 17.6 -> 11.7; one or three pieces from
+// block to block do alike, eight 8.6, 10.8 and 14.7; the tiles above, whose blocks share rows, gain nothing).
+// What bounds it: the weight's bytes and a launch, 16.8 MB in 4.5 us out of the Infinity Cache, 5.7 us out of memory.
 template <int DT, int MB, int NB, int W, int U, bool ANY>
 __global__ __launch_bounds__(64 * W) void k_mat_rows(MatArgs g)
 {
@@ -388,10 +392,12 @@ __global__ __launch_bounds__(64 * W) void k_mat_rows(MatArgs g)
     for (int j = 0; j < 2 * NB; j++) { const unsigned r = j * 8 + (lane >> 3); wr_row[j] = r < nrows ? r : nrows - 1; wo[j] = wr_row[j] * (unsigned)g.w_stride + at; }
 #pragma unroll
     for (int i = 0; i < 2 * MB; i++) { const unsigned r = i * 8 + (lane >> 3); xr_row[i] = r < mrows ? r : mrows - 1; xo[i] = xr_row[i] * (unsigned)g.x_stride + at; }
+    const unsigned pieces = (g.k + 127) / 128, start = blockIdx.x * 3 % pieces;
+    const auto turned = [&](unsigned piece) { const unsigned p = piece + start; return p < pieces ? p : p - pieces; };
     signed char* const ring = smem + wave * RING;
     const auto fetch = [&](unsigned piece, int u) {
-        const unsigned k0 = piece * 128 < g.k ? piece * 128 : 0;       // (within the buffer: the range check subtracts it)
-        const bool past = piece * 128 + at >= g.k;                     // out of the buffer's range: zeros
+        const unsigned k0 = piece < pieces ? turned(piece) * 128 : 0;  // (within the buffer: the range check subtracts it)
+        const bool past = piece >= pieces || k0 + at >= g.k;           // out of the buffer's range: zeros
 #pragma unroll
         for (int j = 0; j < 2 * NB; j++) __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (lds_void*)(ring + u * SLOT + j * 1024), 16, past ? 0x80000000u : wo[j], k0, 0, 0);
 #pragma unroll
@@ -401,7 +407,6 @@ __global__ __launch_bounds__(64 * W) void k_mat_rows(MatArgs g)
 #pragma unroll
     for (int h = 0; h < 2; h++) fo[h] = (lane & 15) * 128 + (((h * 4 + (lane >> 4)) ^ (lane & 7)) << 4);
     i32x4 acc[MB][NB] = {};
-    const unsigned pieces = (g.k + 127) / 128;
     const auto multiply = [&](int u) {
         i32x4 fw[2][NB], fx[2][MB];
 #pragma unroll
@@ -426,15 +431,15 @@ __global__ __launch_bounds__(64 * W) void k_mat_rows(MatArgs g)
         i32x4 next[LOADS];
         const auto load = [&](unsigned piece) {
 #pragma unroll
-            for (int j = 0; j < 2 * NB; j++) next[j] = ask16(g.w + (size_t)(n0 + wr_row[j]) * g.w_stride, piece * 128 + at, g.k);
+            for (int j = 0; j < 2 * NB; j++) next[j] = ask16(g.w + (size_t)(n0 + wr_row[j]) * g.w_stride, turned(piece) * 128 + at, g.k);
 #pragma unroll
-            for (int i = 0; i < 2 * MB; i++) next[2 * NB + i] = ask16(g.x + (size_t)(m0 + xr_row[i]) * g.x_stride, piece * 128 + at, g.k);
+            for (int i = 0; i < 2 * MB; i++) next[2 * NB + i] = ask16(g.x + (size_t)(m0 + xr_row[i]) * g.x_stride, turned(piece) * 128 + at, g.k);
         };
         load(wave);
         for (unsigned p = wave; p < pieces; p += W) {
-            if ((p + 1) * 128 > g.k) {
+            if ((turned(p) + 1) * 128 > g.k) {
 #pragma unroll
-                for (int l = 0; l < LOADS; l++) next[l] = place16(next[l], p * 128 + at, g.k);
+                for (int l = 0; l < LOADS; l++) next[l] = place16(next[l], turned(p) * 128 + at, g.k);
             }
 #pragma unroll
             for (int l = 0; l < LOADS; l++) *(i32x4*)(ring + l * 1024 + lane * 16) = next[l];
@@ -595,23 +600,24 @@ template <int DT> void launch_any(const MatArgs& g, hipStream_t st)
     k_mat_any<DT><<<flat_grid(tiles), 256, 0, st>>>(g);
 }
 
-// The kernels a product of whole 16-byte pieces can take, as tiles: rows of x by rows of w.  What a tile costs on a CU by
-// itself was measured with 256 tiles, one for each CU, k = 4096 and weights from memory: `step` microseconds for each 128
-// bytes of k and `end` for the rest.  Larger tiles read less for each product, smaller ones fill the GPU; an estimate of
-// rounds of 256 tiles x (end + steps x step) decides.  Measured, in us, chosen one first: 16 x 4096 x 4096 16x16 5.5,
-// 32x32 6.5; 64 x 4096 x 4096 32x32 6.5, 64x64 8.9; 128 x 4096 x 4096 64x32 8.2, 64x64 9.0; 256 x 4096 x 4096 64x64 9.9,
-// 128x64 11.8; 512 x 4096 x 4096 128x64 14.4, 128x128 18.7; 1024 x 4096 x 4096 128x128 21.8, 128x64 27.4; 2048 x 4096 x 4096
-// 128x256 36.6, 256x256 44.6; 2048 x 8192 x 4096 256x256 63, 128x128 79.
-struct Tile { unsigned rows, cols; float end, step; bool ring; };
+// The kernels a product of whole 16-byte pieces can take, as tiles: rows of x by rows of w.  `step` is what 128 bytes of k cost
+// with 256 tiles, one for each CU, and `end` the rest, in us, with operands that no cache holds; where a CU holds several blocks
+// at a time (`shared`) they fill one another's gaps and the work counts, otherwise whole rounds of 256 tiles do.  Fitted to 104
+// products of 1 .. 2048 rows by 2048 .. 28672 channels of 1024 .. 14336: the estimate is 14 % (rms) off, the tile it picks within
+// 7 % of the best one of all, with operands in the caches too.  In us, without the caches, chosen one first, channels and k
+// 4096: 16 rows 16x16 5.9, 16x32 6.8; 32 rows 16x32 6.7, 16x16 7.8; 64 rows 32x32 8.0, 16x64 8.8; 128 rows 64x32 10.0, 32x32 10.8;
+// 192 rows 64x64 12.6, 32x32 14.1; 384 rows 128x64 16.7, 64x64 22.6; 1024 rows 128x128 28.0, 128x64 32.4; both 8192: 1024 rows
+// 128x256 71, 128x128 75; 2048 rows 256x256 109, 128x256 138; 16 x 14336 x 4096 16x64 12.6, 16x32 12.7.
+struct Tile { unsigned rows, cols; float end, step; bool ring, shared; };
 constexpr Tile kTiles[] = {
-    {16, 16, 0.7f, 0.07f, true}, {16, 32, 0.4f, 0.09f, true}, {16, 64, 0.6f, 0.18f, true}, {32, 32, 0.4f, 0.097f, true},
-    {64, 32, 0.5f, 0.145f, true}, {64, 64, 1.0f, 0.185f, false}, {128, 64, 1.5f, 0.31f, false}, {128, 128, 2.0f, 0.525f, false},
-    {128, 256, 4.0f, 0.93f, false}, {256, 256, 8.0f, 1.63f, false}};
-// The same for rows that start anywhere.  Measured, in us, chosen one first: 16 x 4096 x 4097 16x16 6.0, 32x32 9.0;
-// 77 x 2741 x 1111 16x32 5.8, 64x64 9.8; 64 x 4096 x 4097 32x32 8.9, 64x64 17.6; 512 x 4096 x 4097 64x64 30.4, 128x128 36.6;
-// 1024 x 4096 x 4097 128x128 38.1, 64x64 55.3.
+    {16, 16, 2.9f, 0.092f, true, true}, {16, 32, 2.4f, 0.127f, true, true}, {16, 64, 1.8f, 0.241f, true, true}, {32, 32, 2.5f, 0.145f, true, true},
+    {64, 32, 2.5f, 0.18f, true, false}, {64, 64, 2.8f, 0.278f, false, false}, {128, 64, 2.7f, 0.41f, false, false}, {128, 128, 2.2f, 0.66f, false, false},
+    {128, 256, 3.2f, 1.0f, false, false}, {256, 256, 9.1f, 1.24f, false, false}};
+// The same for rows that start anywhere (45 products; 14 % and 9 %), 4096 channels of 4097: 16 rows 16x16 7.4, 16x32 9.9; 32 rows
+// 16x32 9.5, 16x16 10.6; 64 rows 32x32 11.3, 16x32 14.0; 256 rows 64x64 21.2, 32x32 29.9; 1024 rows 128x128 42.9, 64x64 59.4.
 constexpr Tile kAnyTiles[] = {
-    {16, 16, 0.3f, 0.085f, true}, {16, 32, 0.4f, 0.14f, true}, {32, 32, 0.5f, 0.165f, true}, {64, 64, 0.8f, 0.42f, true}, {128, 128, 3.0f, 1.05f, false}};
+    {16, 16, 2.7f, 0.105f, true, true}, {16, 32, 2.4f, 0.173f, true, true}, {32, 32, 2.9f, 0.21f, true, true}, {64, 64, 3.2f, 0.489f, true, false},
+    {128, 128, 5.5f, 1.08f, false, false}};
 
 template <int N> int pick_tile(const Tile (&tiles)[N], unsigned m, unsigned n, unsigned k)
 {
@@ -622,7 +628,8 @@ template <int N> int pick_tile(const Tile (&tiles)[N], unsigned m, unsigned n, u
         const Tile& t = tiles[i];
         const size_t tm = ((size_t)m + t.rows - 1) / t.rows, tn = ((size_t)n + t.cols - 1) / t.cols;
         if (t.ring && (tm > 65535 || tn > (1u << 20))) continue;      // a grid's y and x
-        const float us = (float)((tm * tn + 255) / 256) * (t.end + steps * t.step);
+        const float rounds = tm * tn <= 256 ? 1.0f : t.shared ? (float)(tm * tn) / 256 : (float)((tm * tn + 255) / 256);
+        const float us = t.shared ? t.end + rounds * steps * t.step : rounds * (t.end + steps * t.step);
         if (least == 0.0f || us < least) { best = i; least = us; }
     }
     return best;
@@ -648,11 +655,11 @@ template <int DT> void launch_mat(const MatArgs& g, hipStream_t st)
         }
     }
     switch (pick_tile(kTiles, g.m, g.n, g.k)) {
-        case 0: return launch_rows<DT, 1, 1, 16, 2>(g, st);
-        case 1: return launch_rows<DT, 1, 2, 8, 2>(g, st);
-        case 2: return launch_rows<DT, 1, 4, 8, 2>(g, st);
+        case 0: return launch_rows<DT, 1, 1, 8, 2>(g, st);
+        case 1: return launch_rows<DT, 1, 2, 4, 2>(g, st);
+        case 2: return launch_rows<DT, 1, 4, 4, 2>(g, st);
         case 3: return launch_rows<DT, 2, 2, 4, 2>(g, st);
-        case 4: return launch_rows<DT, 4, 2, 8, 1>(g, st);
+        case 4: return launch_rows<DT, 4, 2, 4, 2>(g, st);
         case 5: return launch_tile<DT, 1, 1, 3, 2>(g, st);
         case 6: return launch_tile<DT, 2, 1, 2, 2>(g, st);
         case 7: return launch_tile<DT, 2, 2, 2, 1>(g, st);
