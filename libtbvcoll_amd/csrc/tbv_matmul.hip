@@ -84,7 +84,7 @@ __global__ __launch_bounds__(256) void k_mat_short(MatArgs g)
 // rotated by the row so that the lanes that read a fragment together find it in different banks.  The LDS holds S steps of w
 // and S + 1 of x: step t + S of x is asked for at the start of step t, into the buffer of t - 1, and of w in its middle, once
 // the last fragment of t has been read.  Fragments are read half a step ahead of the products that use them, so a step has
-// one barrier and no product waits for the LDS.  G groups of four waves take the steps in turn and join their sums in the LDS,
+// one barrier and no product waits for the LDS; two blocks share a CU where 80 KB of LDS do for one.  G groups of four waves take the steps in turn and join their sums in the LDS,
 // for products with fewer tiles than the GPU has CUs.
 // What bounds it (2048 x 8192 x 4096 bf16 61 us, 8192 x 8192 x 4096 223 us: 2.25 and 2.46 POP/s, the library's product alone
 // takes 68 and 245): the matrix units, busy 68 % of the cycles, at the clock that the power limit leaves (1.85 GHz; the same
@@ -114,7 +114,7 @@ template <> struct Out<2> { typedef __bf16 T; [[maybe_unused]] static constexpr 
 }
 
 template <int DT, int TM, int TN, int S, int G, bool THROUGH>
-__global__ __launch_bounds__(256 * G, TM * TN >= 8 ? 1 : 2) void k_mat_tile(MatArgs g)
+__global__ __launch_bounds__(256 * G, G * ((S + 1) * TM + S * TN) * 8192 > 81920 ? G : 2 * G) void k_mat_tile(MatArgs g)
 {
 #ifdef __HIP_DEVICE_COMPILE__          // (register constraints and buffer loads the host pass does not know)
     constexpr int BM = 64 * TM, BN = 64 * TN, XS = BM * 128, WS = BN * 128, ESZ = Out<DT>::SIZE;
@@ -602,22 +602,25 @@ template <int DT> void launch_any(const MatArgs& g, hipStream_t st)
 
 // The kernels a product of whole 16-byte pieces can take, as tiles: rows of x by rows of w.  `step` is what 128 bytes of k cost
 // with 256 tiles, one for each CU, and `end` the rest, in us, with operands that no cache holds; where a CU holds several blocks
-// at a time (`shared`) they fill one another's gaps and the work counts, otherwise whole rounds of 256 tiles do.  Fitted to 104
-// products of 1 .. 2048 rows by 2048 .. 28672 channels of 1024 .. 14336: the estimate is 14 % (rms) off, the tile it picks within
-// 7 % of the best one of all, with operands in the caches too.  In us, without the caches, chosen one first, channels and k
-// 4096: 16 rows 16x16 5.9, 16x32 6.8; 32 rows 16x32 6.7, 16x16 7.8; 64 rows 32x32 8.0, 16x64 8.8; 128 rows 64x32 10.0, 32x32 10.8;
-// 192 rows 64x64 12.6, 32x32 14.1; 384 rows 128x64 16.7, 64x64 22.6; 1024 rows 128x128 28.0, 128x64 32.4; both 8192: 1024 rows
-// 128x256 71, 128x128 75; 2048 rows 256x256 109, 128x256 138; 16 x 14336 x 4096 16x64 12.6, 16x32 12.7.
-struct Tile { unsigned rows, cols; float end, step; bool ring, shared; };
+// at a time (`shared`) they fill one another's gaps and the work counts, otherwise whole rounds of 256 tiles do.  128 x 128 comes
+// twice: three steps ahead and a block to a CU where one round does (`once`), two steps ahead and two blocks to a CU beyond
+// (1024 x 4096 x 8192: 41.6 and 50.5; 2048 x 4096 x 4096: 45.2 and 39.7).  Fitted to 138 products of 1 .. 4096 rows by 2048 .. 28672
+// channels of 1024 .. 14336: the estimate is 14 % (rms) off, the tile it picks within 8 % of the best one of all, with operands
+// in the caches too.  In us, without the caches, chosen one first, channels and k 4096: 16 rows 16x16 5.9, 16x32 6.8; 32 rows
+// 16x32 6.7, 16x16 7.8; 64 rows 32x32 8.0, 16x64 8.8; 128 rows 64x32 10.0, 32x32 10.8; 192 rows 64x64 12.7, 128x64 15.7;
+// 384 rows 128x64 17.0, 128x128 21.5; 1024 rows 128x128 24.3 (two steps ahead 28.4); 2048 rows 128x256 38.8, 128x128 41.4;
+// 4096 rows 256x256 61.4, 128x256 75.4; 16 x 14336 x 4096 16x64 12.6, 16x32 12.7.
+struct Tile { unsigned rows, cols; float end, step; bool ring, shared, once; };
 constexpr Tile kTiles[] = {
-    {16, 16, 2.9f, 0.092f, true, true}, {16, 32, 2.4f, 0.127f, true, true}, {16, 64, 1.8f, 0.241f, true, true}, {32, 32, 2.5f, 0.145f, true, true},
-    {64, 32, 2.5f, 0.18f, true, false}, {64, 64, 2.8f, 0.278f, false, false}, {128, 64, 2.7f, 0.41f, false, false}, {128, 128, 2.2f, 0.66f, false, false},
-    {128, 256, 3.2f, 1.0f, false, false}, {256, 256, 9.1f, 1.24f, false, false}};
+    {16, 16, 2.9f, 0.092f, true, true, false}, {16, 32, 2.4f, 0.127f, true, true, false}, {16, 64, 1.8f, 0.241f, true, true, false},
+    {32, 32, 2.4f, 0.158f, true, true, false}, {64, 32, 2.5f, 0.177f, true, false, false}, {64, 64, 2.9f, 0.281f, false, false, false},
+    {128, 64, 2.9f, 0.401f, false, false, false}, {128, 128, 3.1f, 0.574f, false, false, true}, {128, 128, 2.7f, 0.624f, false, false, false},
+    {128, 256, 5.8f, 0.882f, false, false, false}, {256, 256, 9.1f, 1.287f, false, false, false}};
 // The same for rows that start anywhere (45 products; 14 % and 9 %), 4096 channels of 4097: 16 rows 16x16 7.4, 16x32 9.9; 32 rows
 // 16x32 9.5, 16x16 10.6; 64 rows 32x32 11.3, 16x32 14.0; 256 rows 64x64 21.2, 32x32 29.9; 1024 rows 128x128 42.9, 64x64 59.4.
 constexpr Tile kAnyTiles[] = {
-    {16, 16, 2.7f, 0.105f, true, true}, {16, 32, 2.4f, 0.173f, true, true}, {32, 32, 2.9f, 0.21f, true, true}, {64, 64, 3.2f, 0.489f, true, false},
-    {128, 128, 5.5f, 1.08f, false, false}};
+    {16, 16, 2.7f, 0.105f, true, true, false}, {16, 32, 2.4f, 0.173f, true, true, false}, {32, 32, 2.9f, 0.21f, true, true, false}, {64, 64, 3.2f, 0.489f, true, false, false},
+    {128, 128, 5.5f, 1.08f, false, false, false}};
 
 template <int N> int pick_tile(const Tile (&tiles)[N], unsigned m, unsigned n, unsigned k)
 {
@@ -628,6 +631,7 @@ template <int N> int pick_tile(const Tile (&tiles)[N], unsigned m, unsigned n, u
         const Tile& t = tiles[i];
         const size_t tm = ((size_t)m + t.rows - 1) / t.rows, tn = ((size_t)n + t.cols - 1) / t.cols;
         if (t.ring && (tm > 65535 || tn > (1u << 20))) continue;      // a grid's y and x
+        if (t.once && tm * tn > 256) continue;
         const float rounds = tm * tn <= 256 ? 1.0f : t.shared ? (float)(tm * tn) / 256 : (float)((tm * tn + 255) / 256);
         const float us = t.shared ? t.end + rounds * steps * t.step : rounds * (t.end + steps * t.step);
         if (least == 0.0f || us < least) { best = i; least = us; }
@@ -662,8 +666,9 @@ template <int DT> void launch_mat(const MatArgs& g, hipStream_t st)
         case 4: return launch_rows<DT, 4, 2, 4, 2>(g, st);
         case 5: return launch_tile<DT, 1, 1, 3, 2>(g, st);
         case 6: return launch_tile<DT, 2, 1, 2, 2>(g, st);
-        case 7: return launch_tile<DT, 2, 2, 2, 1>(g, st);
-        case 8: return launch_tile<DT, 2, 4, 2, 1>(g, st);
+        case 7: return launch_tile<DT, 2, 2, 3, 1>(g, st);
+        case 8: return launch_tile<DT, 2, 2, 2, 1>(g, st);
+        case 9: return launch_tile<DT, 2, 4, 3, 1>(g, st);
         default: break;
     }
     // A result that the caches do not hold until it is read is stored past them, which leaves them to x and w.  Alone, and with

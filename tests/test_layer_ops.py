@@ -771,6 +771,42 @@ def test_more_threads_than_a_launch_dimension_holds():
     assert torch.equal(codes[1 << 20].cpu(), c[0]) and int((scale != 2.0 ** -126).sum()) == 4
 
 
+# Ragged products that reach each of the product's kernels: few rows 16x16 .. 64x32, tiles 64x64 .. 256x256 (128x128 in its two
+# depths), and the five for rows that start anywhere.
+KERNELS = [(17, 40, 4096), (70, 33, 4000), (17, 40, 1040), (39, 1000, 1040), (7, 40, 144), (500, 8200, 16), (97, 2741, 1040), (333, 1000, 1040),
+           (300, 2741, 272), (130, 4100, 1040), (333, 2741, 272), (1030, 1000, 144), (130, 8200, 1040), (500, 4100, 1040), (777, 2741, 1040),
+           (777, 2741, 16), (2100, 1000, 16), (777, 8200, 144), (2100, 2741, 272), (1030, 8200, 144), (2100, 4100, 1040),
+           (17, 40, 1041), (17, 40, 143), (300, 4100, 17), (777, 1000, 143), (300, 2741, 143), (500, 4100, 1041), (777, 4100, 143)]
+
+
+@gpu
+@pytest.mark.parametrize("name", ["f32", "bf16"])
+@pytest.mark.parametrize("m,n,k", KERNELS, ids=lambda v: str(v))
+def test_every_kernel_of_the_product(m, n, k, name):
+    dt = DT[name]
+    x, w = codes_of(m + k, m, k), codes_of(n + 3 * k, n, k)
+    xs, ws = scales_of(1, m), scales_of(2, n, 0.0005)
+    bias = torch.from_numpy(synth.normal(3, n)).to(dt)
+    say("product", m, n, k, name)
+    out = torch.full((m, n + 8), 7.0, dtype=dt, device="cuda")
+    tbvcoll.matmul_int8(x.cuda(), xs.cuda(), w.cuda(), ws.cuda(), bias=bias.cuda(), out=out[:, :n])
+    want, before = want_product(x, xs, w, ws, bias)
+    check(out[:, :n], want, before, dt, (m, n, k, name))
+    assert bool((out[:, n:] == 7.0).all())
+
+
+@gpu
+@pytest.mark.parametrize("m,n,k", [(4100, 4112, 1040), (5001, 7000, 1008)])
+def test_product_with_a_large_result(m, n, k):
+    """A result that is stored past the caches: every element, and the guards beside the rows."""
+    x, w = codes_of(1, m, k).cuda(), codes_of(2, n, k).cuda()
+    one = torch.ones(1, device="cuda")
+    out = torch.full((m, n + 4), 7.0, device="cuda")
+    say("product", m, n, k)
+    tbvcoll.matmul_int8(x, one, w, one, out=out[:, :n])
+    assert torch.equal(out[:, :n], torch.matmul(x.float(), w.float().t().contiguous())) and bool((out[:, n:] == 7.0).all())     # 1040 * 127^2 < 2^24: exact
+
+
 @gpu
 @pytest.mark.parametrize("m,n", [(1, 1), (2, 1), (1, 3), (17, 1), (40, 2), (130, 1), (300, 300)])
 @pytest.mark.parametrize("k", [16, 32, 144])
