@@ -370,8 +370,9 @@ template <int DT, int TM, int TN, int S, int G, bool THROUGH = false> void launc
 // are often a power of two apart, and with all blocks at one column the loads meet in a few of the caches' and the memory's
 // channels (16 x 8192 x 4096 8.2 -> 7.1 us, 64 x 4096 x 8192 12.5 -> 8.7, 4 x 8192 x 8192 17.6 -> 11.7; one or three pieces from
 // block to block do alike, eight 8.6, 10.8 and 14.7; the tiles above, whose blocks share rows, gain nothing).
-// What bounds it: the weight's bytes and a launch, 16.8 MB in 4.5 us out of the Infinity Cache, 5.7 us out of memory.
-template <int DT, int MB, int NB, int W, int U, bool ANY>
+// What bounds it: the weight's bytes and a launch, 16.8 MB in 4.5 us out of the Infinity Cache, 5.5 us out of memory; 67 MB in
+// 12.5 us out of memory, 6.7 TB/s beyond the launch.
+template <int DT, int MB, int NB, int W, int U, bool ANY, bool ONCE>
 __global__ __launch_bounds__(64 * W) void k_mat_rows(MatArgs g)
 {
 #ifdef __HIP_DEVICE_COMPILE__
@@ -399,7 +400,7 @@ __global__ __launch_bounds__(64 * W) void k_mat_rows(MatArgs g)
         const unsigned k0 = piece < pieces ? turned(piece) * 128 : 0;  // (within the buffer: the range check subtracts it)
         const bool past = piece >= pieces || k0 + at >= g.k;           // out of the buffer's range: zeros
 #pragma unroll
-        for (int j = 0; j < 2 * NB; j++) __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (lds_void*)(ring + u * SLOT + j * 1024), 16, past ? 0x80000000u : wo[j], k0, 0, 0);
+        for (int j = 0; j < 2 * NB; j++) __builtin_amdgcn_raw_ptr_buffer_load_lds(wr, (lds_void*)(ring + u * SLOT + j * 1024), 16, past ? 0x80000000u : wo[j], k0, 0, ONCE ? 2 : 0);
 #pragma unroll
         for (int i = 0; i < 2 * MB; i++) __builtin_amdgcn_raw_ptr_buffer_load_lds(xr, (lds_void*)(ring + u * SLOT + (2 * NB + i) * 1024), 16, past ? 0x80000000u : xo[i], k0, 0, 0);
     };
@@ -495,7 +496,18 @@ __global__ __launch_bounds__(64 * W) void k_mat_rows(MatArgs g)
 
 template <int DT, int MB, int NB, int W, int U, bool ANY = false> void launch_rows(const MatArgs& g, hipStream_t st)
 {
-    k_mat_rows<DT, MB, NB, W, U, ANY><<<dim3((g.n + 16 * NB - 1) / (16 * NB), (g.m + 16 * MB - 1) / (16 * MB)), 64 * W, 0, st>>>(g);
+    const dim3 grid((g.n + 16 * NB - 1) / (16 * NB), (g.m + 16 * MB - 1) / (16 * MB));
+    if constexpr (!ANY) {
+        // A weight that one row of blocks reads, and that the L2s (32 MB) cannot keep for the next call, is loaded past them.  Out
+        // of memory and out of the Infinity Cache: 33.5 MB (16 x 8192 x 4096) 8.1 -> 7.5 and 7.0 -> 6.9 us; 59 MB 12.7 -> 11.6 and
+        // 10.6 -> 10.9; 67 MB 14.3 -> 12.5 and 11.7 -> 12.0; but 16.8 MB 5.5 -> 5.2 and, out of the L2s, 3.7 -> 4.5; with two rows
+        // of blocks (64 x 4096 x 8192) 12.7 -> 12.4 and 8.7 -> 11.8.
+        if (grid.y == 1 && (size_t)g.n * g.k >= ((size_t)32 << 20)) {
+            k_mat_rows<DT, MB, NB, W, U, ANY, true><<<grid, 64 * W, 0, st>>>(g);
+            return;
+        }
+    }
+    k_mat_rows<DT, MB, NB, W, U, ANY, false><<<grid, 64 * W, 0, st>>>(g);
 }
 
 // ------------------------------------------------------------------ tiles of operands of any alignment

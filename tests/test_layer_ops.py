@@ -772,11 +772,11 @@ def test_more_threads_than_a_launch_dimension_holds():
 
 
 # Ragged products that reach each of the product's kernels: few rows 16x16 .. 64x32, tiles 64x64 .. 256x256 (128x128 in its two
-# depths), and the five for rows that start anywhere.
+# depths), few rows with a weight of 32 MB and more, and the five for rows that start anywhere.
 KERNELS = [(17, 40, 4096), (70, 33, 4000), (17, 40, 1040), (39, 1000, 1040), (7, 40, 144), (500, 8200, 16), (97, 2741, 1040), (333, 1000, 1040),
            (300, 2741, 272), (130, 4100, 1040), (333, 2741, 272), (1030, 1000, 144), (130, 8200, 1040), (500, 4100, 1040), (777, 2741, 1040),
            (777, 2741, 16), (2100, 1000, 16), (777, 8200, 144), (2100, 2741, 272), (1030, 8200, 144), (2100, 4100, 1040),
-           (17, 40, 1041), (17, 40, 143), (300, 4100, 17), (777, 1000, 143), (300, 2741, 143), (500, 4100, 1041), (777, 4100, 143)]
+           (3, 8200, 4112), (16, 4100, 8208), (30, 8200, 8208), (1, 28700, 4096), (17, 40, 1041), (17, 40, 143), (300, 4100, 17), (777, 1000, 143), (300, 2741, 143), (500, 4100, 1041), (777, 4100, 143)]
 
 
 @gpu
