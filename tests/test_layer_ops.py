@@ -14,6 +14,7 @@ import itertools
 import os
 import subprocess
 import sys
+import threading
 
 import numpy as np
 import pytest
@@ -707,6 +708,41 @@ def test_layer_ops_in_a_graph_and_on_two_streams():
     torch.cuda.synchronize()
     for a, b in zip(got, eager):
         assert all(torch.equal(u, v) for u, v in zip(a, b))
+
+
+@gpu
+def test_layer_ops_from_two_threads():
+    """Two threads at once, each on a stream of its own: every result is that of the calls made alone."""
+    tokens, heads, head, hidden = 24, 4, 64, 512
+    w, ws = codes_of(80, heads * head, hidden).cuda(), scales_of(81, heads * head, 0.0004).cuda()
+    freqs, _ = tbvcoll.rotary_frequencies(head)
+    pos = torch.arange(tokens, device="cuda")
+    xs = [dev(synth.normal(82 + i, tokens * hidden), torch.bfloat16).view(tokens, hidden) for i in range(2)]
+
+    def steps(x):
+        y = tbvcoll.matmul_int8(*tbvcoll.quantize_int8(x), w, ws).view(tokens, heads, head)
+        return tbvcoll.rotary(y, None, pos, freqs, q_out=torch.empty_like(y))[0]
+
+    want = [steps(x) for x in xs]
+    torch.cuda.synchronize()
+    bad = []
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                got = [steps(xs[i]) for _ in range(60)]
+            stream.synchronize()
+            bad.extend(r for r, y in enumerate(got) if not torch.equal(y, want[i]))
+        except Exception as e:                                                  # a failure in a thread is the test's
+            bad.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not bad
 
 
 FIRST_CALL_IN_A_CAPTURE = r"""
