@@ -552,14 +552,15 @@ def rotary_frequencies(rot: int, base: float = 10000.0, factor: float = 1.0, met
     return freqs.to(device), scale
 
 
-def _heads(t, shape, o, what):
-    """The nine fields of tbv_rotary_heads for t ([tokens, heads, head] or [batch, tokens, heads, head]) turned into o."""
+def _heads(t, shape, o, dtype, dev, what):
+    """The nine fields of tbv_rotary_heads for t ([tokens, heads, head] or [batch, tokens, heads, head], of this type and
+    device) turned into o."""
     s = t.stride()
     if o is None or o is t:
         at = to = t.data_ptr()
         u = s
     else:
-        if o.dtype is not t.dtype or o.get_device() != t.get_device() or o.shape != shape:
+        if o.dtype is not dtype or o.get_device() != dev or o.shape != shape:
             raise ValueError(what + "_out has to be of its input's type, device and shape")
         u, at, to = o.stride(), t.data_ptr(), o.data_ptr()
     if (s[-1] != 1 or u[-1] != 1) and shape[-1] > 1:
@@ -578,23 +579,23 @@ def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, freqs: tor
     [batch, tokens].  freqs: fp64, rot/2 of them (`rotary_frequencies`): the first rot elements of a head turn, the rest
     is copied.  Pairs are (i, i + rot/2), or (2i, 2i + 1) with `interleaved`; cos and sin are multiplied by `scale`.
     `inverse` turns back: with the outputs' gradients for q and k it is the backward pass.  Returns (q_out, k_out)."""
-    dev, shape, code = q.get_device(), q.shape, _DT.get(q.dtype)
-    d = len(shape)
+    dev, shape, dtype = q.get_device(), q.shape, q.dtype
+    d, code = len(shape), _DT.get(dtype)
     if dev < 0 or code is None or (d != 3 and d != 4):
         raise ValueError("q has to be fp32, fp16 or bf16 on the GPU, [tokens, heads, head] or [batch, tokens, heads, head]")
     if q.requires_grad or (k is not None and k.requires_grad):
         _frozen()
     batch, tokens, head = 1 if d == 3 else shape[0], shape[-3], shape[-1]
-    hq = _heads(q, shape, q_out, "q")
+    hq = _heads(q, shape, q_out, dtype, dev, "q")
     if k is None:
         if k_out is not None:
             raise ValueError("k_out without k")
         hk = _NO_HEADS
     else:
         ks = k.shape
-        if k.dtype is not q.dtype or k.get_device() != dev or len(ks) != d or ks[0] != shape[0] or ks[-3] != tokens or ks[-1] != head:
+        if k.dtype is not dtype or k.get_device() != dev or len(ks) != d or ks[0] != shape[0] or ks[-3] != tokens or ks[-1] != head:
             raise ValueError("k has to be of q's type and device and differ in its heads only")
-        hk = _heads(k, ks, k_out, "k")
+        hk = _heads(k, ks, k_out, dtype, dev, "k")
     wide, ps = _WIDE.get(positions.dtype), positions.shape
     if positions.get_device() != dev or wide is None:
         raise ValueError("positions have to be int64 or int32 on q's device")

@@ -878,6 +878,25 @@ def test_tensors_that_ask_for_a_gradient_are_refused():
 
 
 @gpu
+@pytest.mark.parametrize("stride", [1 << 22, (1 << 22) + 16, (1 << 23) + 3])
+@pytest.mark.parametrize("m,n,k", [(3, 40, 272), (300, 2741, 272), (500, 4100, 1040)])
+def test_product_of_rows_far_apart(m, n, k, stride):
+    """Row strides at and beyond what a tile's 32-bit offsets hold, of x, and for few rows of w too."""
+    x, w = codes_of(1, m, k), codes_of(2, n, k)
+    xs, ws = scales_of(3, m), scales_of(4, n)
+    far = torch.zeros((m - 1) * stride + k, dtype=torch.int8, device="cuda").as_strided((m, k), (stride, 1))
+    far.copy_(x)
+    wf = w.cuda()
+    if n < 100:
+        wf = torch.zeros((n - 1) * stride + k, dtype=torch.int8, device="cuda").as_strided((n, k), (stride, 1))
+        wf.copy_(w)
+    say("product", m, n, k, stride)
+    got = tbvcoll.matmul_int8(far, xs.cuda(), wf, ws.cuda(), dtype=torch.float32)
+    want, before = want_product(x, xs, w, ws, None)
+    check(got, want, before, torch.float32, (m, n, k, stride))
+
+
+@gpu
 def test_offsets_beyond_32_bits():
     """Rows beyond 4 GiB of codes, inputs and outputs: the last rows' results are those of the rows alone."""
     k, m = 131056, 33000                                                       # 4.3e9 codes
