@@ -9,6 +9,8 @@
 #include <hip/hip_runtime.h>
 #include <stdio.h>
 
+#include <type_traits>
+
 #include "../../include/tbvcoll.h"
 #include "tbv_device.h"
 #include "tbv_step.h"
@@ -112,10 +114,18 @@ template <int DT> __device__ __forceinline__ void store_codes(signed char* row, 
         const uint32_t lo = __builtin_amdgcn_perm(t[4 * e + 1], t[4 * e], 0x0c0c0400u), hi = __builtin_amdgcn_perm(t[4 * e + 3], t[4 * e + 2], 0x04000c0cu);
         o[e] = fine ? lo | hi : 0u;
     }
-    // (Ordinary stores: non-temporal ones make the kernel itself faster, 8.2 -> 6.6 us at 2048 x 4096 bf16, but the product
-    // that reads the codes next then finds them in no cache: with a multiply by the scales behind it 30.5 -> 33.4 us.)
-    if ((j + 1) * N <= hidden) __builtin_memcpy(row + (size_t)j * N, o, N);
-    else for (unsigned e = 0; j * N + e < hidden; e++) row[(size_t)j * N + e] = (signed char)(o[e >> 2] >> (8 * (e & 3)));
+    // Whole vectors are written through the L2 (a relaxed store of agent scope): lines that are still dirty when the kernel
+    // ends stand between it and the next one.  2048 x 4096 bf16 9.0 -> 7.9 us, with the product of the codes behind it 45.8 -> 44.5;
+    // non-temporal ones, which the Infinity Cache does not keep, 7.7 and 45.2, with a copy behind 12.6 against 11.8 (ordinary: 12.7).
+    typedef typename std::conditional<N == 8, unsigned long long, uint32_t>::type T;
+    signed char* const to = row + (size_t)j * N;
+    if ((j + 1) * N <= hidden) {
+        T v;
+        __builtin_memcpy(&v, o, N);
+        if (((uintptr_t)to & (N - 1)) == 0) __hip_atomic_store((T*)to, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        else __builtin_memcpy(to, &v, N);
+    }
+    else for (unsigned e = 0; j * N + e < hidden; e++) to[e] = (signed char)(o[e >> 2] >> (8 * (e & 3)));
 }
 
 struct RowScale { float s, inv; bool fine; };
@@ -129,7 +139,8 @@ template <int DT> __device__ __forceinline__ RowScale row_scale(uint32_t top)
 
 struct RowsArgs { signed char* codes; float* scale; const char* x; size_t code_stride, x_stride; unsigned rows, hidden; };   // x_stride in bytes
 
-// A row is held in registers, read once: R rows to a block, L lanes to a row, V vectors to a lane (L > 64: one row).
+// A row is held in registers, read once: R rows to a block, L lanes to a row, V vectors to a lane (L > 64: one row).  What
+// bounds it: memory and a launch, 25 MB (2048 x 4096 bf16) in 7.0 us out of the Infinity Cache, 7.9 us out of memory.
 template <int DT, int L, int V>
 __global__ __launch_bounds__(L <= 64 ? 256 : L) void k_quant_rows(RowsArgs g)
 {

@@ -113,7 +113,7 @@ template <> struct Out<2> { typedef __bf16 T; [[maybe_unused]] static constexpr 
     return true;
 }
 
-template <int DT, int TM, int TN, int S, int G, bool THROUGH>
+template <int DT, int TM, int TN, int S, int G, bool PAST>
 __global__ __launch_bounds__(256 * G, G * ((S + 1) * TM + S * TN) * 8192 > 81920 ? G : 2 * G) void k_mat_tile(MatArgs g)
 {
 #ifdef __HIP_DEVICE_COMPILE__          // (register constraints and buffer loads the host pass does not know)
@@ -305,7 +305,7 @@ __global__ __launch_bounds__(256 * G, G * ((S + 1) * TM + S * TN) * 8192 > 81920
         }
     signed char* const strip = smem + 2 * BN * 4 + (group * 4 + wave) * 32 * PITCH;
     const unsigned nw = n0 + wn, cols = nw >= g.n ? 0 : g.n - nw < 32 * TN ? g.n - nw : 32 * TN;
-    const bool aligned = (((uintptr_t)g.out | (g.out_stride * ESZ)) & 15) == 0, whole = aligned && cols == 32 * TN;
+    const bool aligned = (((uintptr_t)g.out | (g.out_stride * ESZ)) & 15) == 0, whole = aligned && cols == 32 * TN && g.out_stride < (1u << 25);   // (32 rows: 32-bit offsets)
 #pragma unroll
     for (int i = 0; i < TM; i++) {
         if (G > 1 && (int)group != owner(i)) continue;
@@ -326,13 +326,14 @@ __global__ __launch_bounds__(256 * G, G * ((S + 1) * TM + S * TN) * 8192 > 81920
         __builtin_amdgcn_wave_barrier();
         T* const o = (T*)g.out + (size_t)ms * g.out_stride + nw;
         if (whole && ms + 32 <= g.m) {
+            // written through the L2 (agent scope): lines that are still dirty when the kernel ends stand between it and the next
+            const __amdgpu_buffer_rsrc_t to = __builtin_amdgcn_make_buffer_rsrc(o, 0, 0xffffffff, 0x00020000);
 #pragma unroll
             for (int u = 0; u < VPR / 2; u++) {
                 const unsigned v = u * 64 + lane, row = v / VPR, col = v % VPR * EPV;
                 const u32x4 d = *(const u32x4*)(strip + row * PITCH + col * ESZ);
-                u32x4* const to = (u32x4*)(o + row * g.out_stride + col);
-                if (THROUGH) __builtin_nontemporal_store(d, to);
-                else *to = d;
+                if (PAST) __builtin_nontemporal_store(d, (u32x4*)(o + row * g.out_stride + col));
+                else __builtin_amdgcn_raw_buffer_store_b128(d, to, (unsigned)((row * g.out_stride + col) * ESZ), 0, 16);
             }
         } else if (aligned) {                         // the last tiles: whole vectors up to the edge
 #pragma unroll 2
@@ -355,10 +356,10 @@ __global__ __launch_bounds__(256 * G, G * ((S + 1) * TM + S * TN) * 8192 > 81920
 #endif
 }
 
-template <int DT, int TM, int TN, int S, int G, bool THROUGH = false> void launch_tile(const MatArgs& g, hipStream_t st)
+template <int DT, int TM, int TN, int S, int G, bool PAST = false> void launch_tile(const MatArgs& g, hipStream_t st)
 {
     const size_t tiles = (size_t)((g.m + 64 * TM - 1) / (64 * TM)) * ((g.n + 64 * TN - 1) / (64 * TN));
-    k_mat_tile<DT, TM, TN, S, G, THROUGH><<<flat_grid(tiles), 256 * G, 0, st>>>(g);
+    k_mat_tile<DT, TM, TN, S, G, PAST><<<flat_grid(tiles), 256 * G, 0, st>>>(g);
 }
 
 // ------------------------------------------------------------------ few rows of x: the weights' bytes are the work
@@ -683,9 +684,10 @@ template <int DT> void launch_mat(const MatArgs& g, hipStream_t st)
         case 9: return launch_tile<DT, 2, 4, 3, 1>(g, st);
         default: break;
     }
-    // A result that the caches do not hold until it is read is stored past them, which leaves them to x and w.  Alone, and with
-    // a copy of the result behind the product: 134 MB (8192 x 8192 bf16, k = 4096) 230 -> 223 and 276 -> 270 us; 34 MB
-    // (2048 x 8192) 61 -> 59, but 69 -> 72.
+    // A result that the caches do not hold until it is read is stored past them, others are written through the L2.  Ordinary
+    // stores, through, past, alone and with a copy of the result behind the product, in us: 17 MB (2048 x 4096 bf16, k = 4096) 36.8,
+    // 36.1, 36.6 and 42.8, 42.1, 44.1; 34 MB (2048 x 8192) 60.8, 59.1, 59.6 and 70.6, 68.7, 72.7; 134 MB (8192 x 8192) 233, 232, 227
+    // and 287, 285, 282.
     if ((size_t)g.m * g.n * Out<DT>::SIZE >= ((size_t)64 << 20)) return launch_tile<DT, 4, 4, 2, 1, true>(g, st);
     launch_tile<DT, 4, 4, 2, 1>(g, st);
 }
