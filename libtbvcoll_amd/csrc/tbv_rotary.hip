@@ -34,7 +34,8 @@ struct RotArgs {
     unsigned tokens, head, half, pos64;
     float scale;
     int inverse;
-    bool through;                               // store non-temporally
+    char* base;                                 // of the results
+    bool through;                               // write them through the L2
 };
 
 template <int DT> __device__ __forceinline__ float rot_load(const void* p, ptrdiff_t i)
@@ -125,11 +126,18 @@ template <> struct Lanes<0> {
 };
 
 __device__ __forceinline__ u32x4 load16(const char* p) { u32x4 v; __builtin_memcpy(&v, p, 16); return v; }
-typedef uint32_t u32x4_any __attribute__((ext_vector_type(4), aligned(2)));
-template <bool THROUGH> __device__ __forceinline__ void store16(char* p, u32x4 v)
+// Results are stored in the ordinary way, or written through the L2 (agent scope; addresses are 32-bit offsets from `base` and
+// multiples of 16).
+template <bool THROUGH> __device__ __forceinline__ void store16([[maybe_unused]] char* base, char* p, u32x4 v)
 {
-    if (THROUGH) __builtin_nontemporal_store((u32x4_any)v, (u32x4_any*)p);
-    else __builtin_memcpy(p, &v, 16);
+#ifdef __HIP_DEVICE_COMPILE__
+    if constexpr (THROUGH) {
+        const __amdgpu_buffer_rsrc_t to = __builtin_amdgcn_make_buffer_rsrc(base, 0, 0xffffffff, 0x00020000);
+        __builtin_amdgcn_raw_buffer_store_b128(v, to, (uint32_t)(p - base), 0, 16);
+        return;
+    }
+#endif
+    __builtin_memcpy(p, &v, 16);
 }
 
 template <int DT, bool INTER, int U, bool THROUGH>
@@ -193,7 +201,7 @@ __global__ __launch_bounds__(512) void k_rotary(RotArgs g, unsigned total)
                             p[2 * e] = x[2 * e] * w[e].x - x[2 * e + 1] * w[e].y;
                             p[2 * e + 1] = x[2 * e + 1] * w[e].x + x[2 * e] * w[e].y;
                         }
-                        store16<THROUGH>(out[u] + i * 16, Lanes<DT>::pack(p));
+                        store16<THROUGH>(g.base, out[u] + i * 16, Lanes<DT>::pack(p));
                     } else {
                         Lanes<DT>::unpack(b[u], y);
 #pragma unroll
@@ -201,8 +209,8 @@ __global__ __launch_bounds__(512) void k_rotary(RotArgs g, unsigned total)
                             p[e] = x[e] * w[e].x - y[e] * w[e].y;
                             q[e] = y[e] * w[e].x + x[e] * w[e].y;
                         }
-                        store16<THROUGH>(out[u] + i * 16, Lanes<DT>::pack(p));
-                        store16<THROUGH>(out[u] + i * 16 + apart, Lanes<DT>::pack(q));
+                        store16<THROUGH>(g.base, out[u] + i * 16, Lanes<DT>::pack(p));
+                        store16<THROUGH>(g.base, out[u] + i * 16 + apart, Lanes<DT>::pack(q));
                     }
                 }
             } else if (i < pairs) {
@@ -221,7 +229,7 @@ __global__ __launch_bounds__(512) void k_rotary(RotArgs g, unsigned total)
 #pragma unroll
                 for (int u = 0; u < U; u++) {
                     if (u >= live || out[u] == in[u]) continue;
-                    if (i < vecs) store16<THROUGH>(out[u] + (2 * g.half + (i - pairs) * N) * ESZ, a[u]);
+                    if (i < vecs) store16<THROUGH>(g.base, out[u] + (2 * g.half + (i - pairs) * N) * ESZ, a[u]);
                     else { const unsigned e = 2 * g.half + (rest / N) * N + i - vecs; rot_copy<DT>(out[u], e, in[u], e); }
                 }
             }
@@ -399,11 +407,25 @@ extern "C" int tbv_step_rotary(const tbv_rotary* c, void* stream)
     g.tokens = (unsigned)c->tokens; g.head = (unsigned)c->head; g.half = (unsigned)(c->rot / 2); g.pos64 = c->pos64 != 0;
     g.scale = c->scale; g.inverse = c->inverse != 0;
     const unsigned blocks = (unsigned)(c->batch * c->tokens);
-    // Results that fit the Infinity Cache but not the L2s are written past these: what is still there when the kernel ends
-    // stands between it and the next one.  Alone, and with a copy of the result behind it: 21 MB (2048 tokens of 40 heads of
-    // 128 bf16) 11.7 -> 8.7 and 18.2 -> 17.7 us; 5 MB 5.6 -> 5.0 and 8.4 -> 8.7; 84 MB 35.8 -> 35.5 and 63.5 -> 65.1.
+    // Results are written through the L2 where they are whole lines of 128 bytes and fit the caches: lines that are still dirty
+    // when the kernel ends stand between it and the next.  Ordinary and through, alone and with a copy of the result behind, in
+    // us, operands out of memory: 5 MiB (512 tokens of 40 heads of 128 bf16) 5.7, 5.3 and 8.3, 8.0; 20 MiB 11.7, 10.6 and 18.1, 17.1;
+    // 40 MiB 22.0, 21.0 and 33.3, 32.8; but 80 MiB 36.0, 37.2 and 64.6, 70.4, and heads of 320 bytes (1021 tokens of 20) 6.1, 6.7 and
+    // 8.9, 9.5.  (Non-temporal ones, which the Infinity Cache does not keep: 20 MiB 8.7 alone, 17.7 with the copy, 16.9 instead of 14.9
+    // where the caches hold the operands.)
     const size_t result = (size_t)blocks * (size_t)(c->q.heads + c->k.heads) * (size_t)c->head * esz;
-    g.through = result >= ((size_t)16 << 20) && result <= ((size_t)64 << 20);
+    uintptr_t lo = UINTPTR_MAX, hi = 0;
+    size_t starts = (size_t)c->rot * esz | (size_t)c->head * esz;    // of what is stored, in bytes
+    if (!c->interleaved) starts |= (size_t)c->rot / 2 * esz;
+    for (int i = 0; i < 2; i++) {
+        if (!g.h[i].heads) continue;
+        if (spans_out[i].lo < lo) lo = spans_out[i].lo;
+        if (spans_out[i].hi > hi) hi = spans_out[i].hi;
+        starts |= (uintptr_t)g.h[i].out;
+        for (int j = 0; j < 3; j++) starts |= (size_t)outs[i].stride[j] * esz;
+    }
+    g.base = (char*)lo;
+    g.through = (starts & 127) == 0 && result <= ((size_t)64 << 20) && hi - lo < ((size_t)1 << 32);
     hipStream_t st = (hipStream_t)stream;
     switch (c->dtype) {
         case 0: launch_rot<0>(g, c->interleaved != 0, blocks, st); break;
