@@ -86,7 +86,7 @@ __global__ __launch_bounds__(256) void k_mat_short(MatArgs g)
 // the last fragment of t has been read.  Fragments are read half a step ahead of the products that use them, so a step has
 // one barrier and no product waits for the LDS; two blocks share a CU where 80 KB of LDS do for one.  G groups of four waves take the steps in turn and join their sums in the LDS,
 // for products with fewer tiles than the GPU has CUs.
-// What bounds it (2048 x 8192 x 4096 bf16 61 us, 8192 x 8192 x 4096 224 us: 2.24 and 2.45 POP/s, the library's product alone
+// What bounds it (2048 x 8192 x 4096 bf16 61 us, 8192 x 8192 x 4096 217-232 us: 2.24 and 2.4-2.5 POP/s, the library's product alone
 // takes 68 and 245): the matrix units, busy 68 % of the cycles, at the clock that the power limit leaves (1.85 GHz; the same
 // product of zeros takes three quarters of the time).
 typedef __attribute__((address_space(3))) void lds_void;
