@@ -517,6 +517,10 @@ def test_rotary_inverse_is_the_gradient(interleaved):
 @gpu
 @pytest.mark.parametrize("interleaved", [False, True])
 def test_rotary_in_an_autograd_function(interleaved):
+    in_a_process_of_its_own("autograd_function", interleaved)
+
+
+def autograd_function(interleaved):
     """The backward pass as a training program has it, a shared (expanded) key head among the inputs, against autograd
     through the plain formula in 64 bits on the CPU; captured into a graph with leaves of its own."""
     t, hq, hk, d, scale = 5, 4, 2, 32, 1.25
@@ -556,6 +560,29 @@ def test_rotary_in_an_autograd_function(interleaved):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(caught[0], eager[0]) and torch.equal(caught[1], eager[1])
+
+
+@gpu
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("apart", [(3 << 30) + 4096, (4 << 30) - 16 * 512, (4 << 30) - 8 * 512, 5 << 30])
+def test_rotary_outputs_far_apart(interleaved, apart):
+    """Outputs of q and k at two places of one buffer, below and beyond what a 32-bit offset reaches; what is around them
+    stays as it was."""
+    t, hq, hk, d = 8, 4, 2, 128
+    q, k = (dev(synth.normal(i, t * h * d), torch.bfloat16).view(t, h, d) for i, h in ((1, hq), (2, hk)))
+    buf = torch.zeros(apart // 2 + 16384, dtype=torch.bfloat16, device="cuda")
+    for first, second in (("q", "k"), ("k", "q")):
+        buf.zero_()
+        at = {first: 4096, second: apart // 2 + 4096}
+        q_out, k_out = (buf[at[n]:at[n] + t * h * d].view(t, h, d) for n, h in (("q", hq), ("k", hk)))
+        pos, (freqs, _) = torch.arange(t, device="cuda") * 1000, tbvcoll.rotary_frequencies(d)
+        say("rotary", apart, first)
+        tbvcoll.rotary(q, k, pos, freqs, interleaved=interleaved, q_out=q_out, k_out=k_out)
+        for x, o in ((q, q_out), (k, k_out)):
+            want, tol = want_rotary(x[None], pos[None], freqs, 1.0, interleaved, False)
+            check(o, want[0], tol[0], torch.bfloat16, (apart, first))
+        q_out.zero_(), k_out.zero_()
+        assert int(torch.count_nonzero(buf)) == 0
 
 
 @gpu
@@ -665,8 +692,22 @@ def test_intercept_row_linear():
         tbvcoll.shutdown()
 
 
+def in_a_process_of_its_own(name, *args):
+    """Streams, once made, stay for the life of a process, which multiplexes them onto a few hardware queues: work on streams
+    of its own runs in a child, so that the tests of the all-reduce's streams find the process as it was without it."""
+    say(name, *args, "in a process of its own")
+    code = f"import sys; sys.path[:0] = [{ROOT!r}, {os.path.join(ROOT, 'tests')!r}]; import test_layer_ops as t; t.{name}(*{args!r}); print('DONE', flush=True)"
+    p = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=240)
+    assert "DONE" in p.stdout, (p.returncode, p.stdout[-1000:], p.stderr[-3000:])
+
+
 @gpu
-def test_layer_ops_in_a_graph_and_on_two_streams():
+@pytest.mark.parametrize("work", ["graph_and_two_streams", "two_threads"])
+def test_layer_ops_on_streams(work):
+    in_a_process_of_its_own(work)
+
+
+def graph_and_two_streams():
     """Captured once and replayed with new inputs and the program's own work in between; the same calls on two streams at
     once, eagerly and as two graphs replayed side by side (nothing is shared between calls)."""
     tokens, heads, kv, head, hidden = 40, 4, 2, 64, 256
@@ -710,8 +751,7 @@ def test_layer_ops_in_a_graph_and_on_two_streams():
         assert all(torch.equal(u, v) for u, v in zip(a, b))
 
 
-@gpu
-def test_layer_ops_from_two_threads():
+def two_threads():
     """Two threads at once, each on a stream of its own: every result is that of the calls made alone."""
     tokens, heads, head, hidden = 24, 4, 64, 512
     w, ws = codes_of(80, heads * head, hidden).cuda(), scales_of(81, heads * head, 0.0004).cuda()
