@@ -362,16 +362,14 @@ def all_reduce_rmsnorm(t: torch.Tensor, weight: torch.Tensor, eps: float, out: t
 # ------------------------------------------------------------------ the layer around the all-reduce (additive)
 #
 # These need no `init` and have nothing to fall back to: a call they cannot take raises ValueError.  They run on the
-# current stream of the tensors' device and record no gradient.  A decode step makes hundreds of these calls, each on the GPU for a few
-# microseconds, so they look at every attribute once and hand the library one packed structure.
+# current stream of the tensors' device and record no gradient.  A decode step makes hundreds of these calls, each on
+# the GPU for a few microseconds, so they look at every attribute once and hand the library one packed structure.
 
 _step_lib = None
 _QUANTIZE = struct.Struct("3P5q")          # tbv_quantize_i8
 _MATMUL = struct.Struct("6P9q")            # tbv_matmul_i8
 _ROTARY = struct.Struct("2P7q2P7q2P10qf4x")  # tbv_rotary
-
-
-_WIDE = {torch.int64: 1, torch.int32: 0}
+_WIDE = {torch.int64: 1, torch.int32: 0}    # positions
 _NO_HEADS = (0,) * 9
 
 
