@@ -362,7 +362,9 @@ def all_reduce_rmsnorm(t: torch.Tensor, weight: torch.Tensor, eps: float, out: t
 # ------------------------------------------------------------------ the layer around the all-reduce (additive)
 #
 # These need no `init` and have nothing to fall back to: a call they cannot take raises ValueError.  They run on the
-# current stream of the tensors' device and record no gradient.  A decode step makes hundreds of these calls, each on
+# current stream of the tensors' device and record no gradient.  They write through raw pointers, so they tell autograd
+# which of the caller's tensors they wrote (`_wrote`: a backward pass that had saved one then raises, as after any other
+# in-place operation).  A decode step makes hundreds of these calls, each on
 # the GPU for a few microseconds, so they look at every attribute once and hand the library one packed structure.
 
 _step_lib = None
@@ -371,6 +373,7 @@ _MATMUL = struct.Struct("6P9q")            # tbv_matmul_i8
 _ROTARY = struct.Struct("2P7q2P7q2P10qf4x")  # tbv_rotary
 _WIDE = {torch.int64: 1, torch.int32: 0}    # positions
 _NO_HEADS = (0,) * 9
+_wrote = torch._C._increment_version         # (of each tensor in a sequence; 0.4 us, the public wrapper 0.6)
 
 
 def _steps():
@@ -430,6 +433,7 @@ def quantize_int8(x: torch.Tensor, codes: torch.Tensor = None, scale: torch.Tens
     if x.requires_grad:
         _frozen()
     rows, cols, xs = _rows(x, shape, "x")
+    given = () if codes is None and scale is None else [t for t in (codes, scale) if t is not None]
     if codes is None:
         codes = torch.empty_like(x, dtype=torch.int8) if x.is_contiguous() else x.new_empty(shape, dtype=torch.int8)
         cs = cols
@@ -443,6 +447,8 @@ def quantize_int8(x: torch.Tensor, codes: torch.Tensor = None, scale: torch.Tens
         raise ValueError("scale has to be contiguous fp32, of x's shape without its last dimension, on its device")
     if rows:
         _launch((_step_lib or _steps()).tbv_step_quantize_i8, dev, _QUANTIZE.pack(codes.data_ptr(), scale.data_ptr(), x.data_ptr(), cs, xs, rows, cols, code))
+        if given:
+            _wrote(given)
     return codes, scale
 
 
@@ -471,9 +477,10 @@ def matmul_int8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale
         code, os_ = _DT.get(dtype), n
         if code is None:
             raise ValueError("the result is fp32, fp16 or bf16")
+        given = False
         out = x_scale.new_empty((m, n) if len(shape) == 2 else shape[:-1] + (n,), dtype=dtype)
     else:
-        dtype = out.dtype
+        dtype, given = out.dtype, True
         code = _DT.get(dtype)
         if code is None:
             raise ValueError("the result is fp32, fp16 or bf16")
@@ -490,6 +497,8 @@ def matmul_int8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale
     if m and n:
         _launch((_step_lib or _steps()).tbv_step_matmul_i8, dev, _MATMUL.pack(
             out.data_ptr(), x.data_ptr(), x_scale.data_ptr(), w.data_ptr(), w_scale.data_ptr(), b, os_, xs, ws, m, n, k, sx, sw, code))
+        if given:
+            _wrote((out,))
     return out
 
 
@@ -608,7 +617,15 @@ def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, freqs: tor
         raise ValueError("freqs has to be contiguous fp64 on q's device, at most half a head and 4096 long")
     _launch((_step_lib or _steps()).tbv_step_rotary, dev, _ROTARY.pack(
         *hq, *hk, positions.data_ptr(), freqs.data_ptr(), p0, p1, batch, tokens, head, rot, code, wide, interleaved, inverse, scale))
-    return q if q_out is None else q_out, k if k_out is None else k_out
+    if q_out is None:
+        q_out = q
+    if k is None:
+        _wrote((q_out,))
+        return q_out, None
+    if k_out is None:
+        k_out = k
+    _wrote((q_out, k_out))
+    return q_out, k_out
 
 
 def shutdown():

@@ -1,0 +1,113 @@
+"""What the layer's operators tell autograd.  They write through raw pointers, so they have to say which of the caller's
+tensors they wrote: a backward pass that had saved one must raise, as after any other in-place operation, not use the
+overwritten values.
+
+The CPU tests give the calls tensors that say they lie on a GPU and take the launch away: what is looked at is what the
+call does before and after it."""
+import pytest
+import torch
+
+from gpu_util import say
+from libtbvcoll_amd import tbvcoll
+
+gpu = pytest.mark.gpu
+
+
+class Stand(torch.Tensor):
+    def get_device(self):
+        return 0
+
+
+def stand(*shape, dtype=torch.float32):
+    return torch.ones(*shape, dtype=dtype).as_subclass(Stand)
+
+
+@pytest.fixture
+def launches(monkeypatch):
+    """The launches that would have been made, by name."""
+    names = []
+    monkeypatch.setattr(tbvcoll, "_launch", lambda fn, device, call: names.append(fn.__name__))
+    return names
+
+
+def on_gpu(*shape, dtype=torch.float32):
+    return torch.ones(*shape, dtype=dtype, device="cuda")
+
+
+def writing_calls(new):
+    """(name, call, tensors of the caller's that it writes), tensors from `new`."""
+    x, q, k = new(4, 16), new(4, 2, 16), new(4, 1, 16)
+    x8, w8, s, s1 = new(4, 16, dtype=torch.int8), new(8, 16, dtype=torch.int8), new(8), new(4)
+    pos, freqs = new(4, dtype=torch.int64), new(8, dtype=torch.float64)
+    codes, scale, out, q_out, k_out = new(4, 16, dtype=torch.int8), new(4), new(4, 8, dtype=torch.bfloat16), new(4, 2, 16), new(4, 1, 16)
+    return [("codes", lambda: tbvcoll.quantize_int8(x, codes=codes), [codes]),
+            ("scale", lambda: tbvcoll.quantize_int8(x, scale=scale), [scale]),
+            ("codes and scale", lambda: tbvcoll.quantize_int8(x, codes, scale), [codes, scale]),
+            ("product", lambda: tbvcoll.matmul_int8(x8, s1, w8, s, out=out), [out]),
+            ("q in place", lambda: tbvcoll.rotary(q, None, pos, freqs), [q]),
+            ("q and k in place", lambda: tbvcoll.rotary(q, k, pos, freqs), [q, k]),
+            ("q out, k in place", lambda: tbvcoll.rotary(q, k, pos, freqs, q_out=q_out), [q_out, k]),
+            ("both out", lambda: tbvcoll.rotary(q, k, pos, freqs, q_out=q_out, k_out=k_out), [q_out, k_out])], \
+        [x, q, k, x8, w8, s, s1, pos, freqs, codes, scale, out, q_out, k_out]
+
+
+def versions(new):
+    """Every call moves the version of exactly the tensors that it wrote."""
+    calls, tensors = writing_calls(new)
+    for name, call, wrote in calls:
+        say("versions", name)
+        before = [t._version for t in tensors]
+        call()
+        moved = [t._version > b for t, b in zip(tensors, before)]
+        assert moved == [any(t is w for w in wrote) for t in tensors], name
+
+
+def test_written_tensors_move_on(launches):
+    versions(stand)
+    assert set(launches) == {"tbv_step_quantize_i8", "tbv_step_matmul_i8", "tbv_step_rotary"}
+
+
+def test_inference_tensors_have_no_version(launches):
+    with torch.inference_mode():
+        for _, call, _ in writing_calls(stand)[0]:
+            call()
+    assert len(launches) == 8
+
+
+@gpu
+def test_written_tensors_move_on_gpu():
+    versions(on_gpu)
+
+
+@gpu
+@pytest.mark.parametrize("how", ["in place", "a view in place", "an output", "under no_grad"])
+def test_backward_notices_a_saved_tensor_that_was_turned(how):
+    """q needs no gradient, but its product with a learned tensor saved it for the backward pass."""
+    q, p = torch.randn(4, 2, 16, device="cuda"), torch.ones(4, 2, 16, device="cuda", requires_grad=True)
+    pos, freqs = torch.arange(4, device="cuda"), torch.ones(8, dtype=torch.float64, device="cuda")
+    y = (q * p).sum()
+    say("rotary after a product saved q:", how)
+    if how == "in place":
+        tbvcoll.rotary(q, None, pos, freqs)
+    elif how == "a view in place":
+        tbvcoll.rotary(q[1:3], None, pos[:2], freqs)
+    elif how == "an output":
+        tbvcoll.rotary(torch.ones_like(q), None, pos, freqs, q_out=q)
+    else:
+        with torch.no_grad():
+            tbvcoll.rotary(q, None, pos, freqs)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+@gpu
+def test_backward_notices_a_saved_result_buffer():
+    """A result buffer that is used again, saved by the step before."""
+    x, w = (torch.ones(n, 16, dtype=torch.int8, device="cuda") for n in (4, 8))
+    one, p = torch.ones(1, device="cuda"), torch.ones(4, 8, device="cuda", requires_grad=True)
+    out = tbvcoll.matmul_int8(x, one, w, one, dtype=torch.float32)
+    y = (out * p).sum()
+    say("product into a saved result")
+    tbvcoll.matmul_int8(x, one, w, one, out=out)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
