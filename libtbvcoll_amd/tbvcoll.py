@@ -400,7 +400,7 @@ def _launch(fn, device, call):
 
 
 def _frozen():
-    """A tensor that requires a gradient: the kernels record none, so the call is for code that asks for none."""
+    """A tensor, read or written, that requires a gradient: the kernels record none, so the call is for code that asks for none."""
     if torch.is_grad_enabled():
         raise ValueError("records no gradient: call it under torch.no_grad(), or in the forward and backward of a torch.autograd.Function")
 
@@ -445,6 +445,8 @@ def quantize_int8(x: torch.Tensor, codes: torch.Tensor = None, scale: torch.Tens
         scale = x.new_empty(shape[:-1], dtype=torch.float32)
     elif scale.dtype is not torch.float32 or scale.shape != shape[:-1] or scale.get_device() != dev or not scale.is_contiguous():
         raise ValueError("scale has to be contiguous fp32, of x's shape without its last dimension, on its device")
+    elif scale.requires_grad:
+        _frozen()
     if rows:
         _launch((_step_lib or _steps()).tbv_step_quantize_i8, dev, _QUANTIZE.pack(codes.data_ptr(), scale.data_ptr(), x.data_ptr(), cs, xs, rows, cols, code))
         if given:
@@ -487,6 +489,8 @@ def matmul_int8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale
         wide = shape[:-1] + (n,)
         if out.get_device() != dev or out.shape != wide:
             raise ValueError("out has to be on x's device, of x's shape with n columns")
+        if out.requires_grad:
+            _frozen()
         os_ = _rows(out, wide, "out")[2]
     if bias is None:
         b = 0
@@ -569,6 +573,8 @@ def _heads(t, shape, o, dtype, dev, what):
     else:
         if o.dtype is not dtype or o.get_device() != dev or o.shape != shape:
             raise ValueError(what + "_out has to be of its input's type, device and shape")
+        if o.requires_grad:
+            _frozen()
         u, at, to = o.stride(), t.data_ptr(), o.data_ptr()
     if (s[-1] != 1 or u[-1] != 1) and shape[-1] > 1:
         raise ValueError(what + ": the elements of a head have to be contiguous")

@@ -111,3 +111,32 @@ def test_backward_notices_a_saved_result_buffer():
     tbvcoll.matmul_int8(x, one, w, one, out=out)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.backward()
+
+
+def outputs_that_ask(new):
+    """Calls into outputs that require a gradient (fp32 ones; codes are integers and cannot)."""
+    def leaf(*shape, dtype=torch.float32):
+        return new(*shape, dtype=dtype).requires_grad_()
+    x, q, k, x8, w8, s, s1, pos, freqs = writing_calls(new)[1][:9]
+    out, q_out, k_out = leaf(4, 8, dtype=torch.bfloat16), leaf(4, 2, 16), leaf(4, 1, 16)
+    return [lambda: tbvcoll.quantize_int8(x, scale=leaf(4)), lambda: tbvcoll.matmul_int8(x8, s1, w8, s, out=out),
+            lambda: tbvcoll.matmul_int8(x8, s1, w8, s, out=out[:, :]),                                    # a view of such a leaf
+            lambda: tbvcoll.rotary(q, k, pos, freqs, q_out=q_out), lambda: tbvcoll.rotary(q, k, pos, freqs, k_out=k_out)]
+
+
+def test_outputs_that_ask_for_a_gradient_are_refused(launches):
+    for call in outputs_that_ask(stand):
+        with pytest.raises(ValueError, match="gradient"):
+            call()
+    assert not launches
+    with torch.no_grad():
+        for call in outputs_that_ask(stand):
+            call()
+    assert len(launches) == 5
+
+
+@gpu
+def test_outputs_that_ask_for_a_gradient_are_refused_on_gpu():
+    for call in outputs_that_ask(on_gpu):
+        with pytest.raises(ValueError, match="gradient"):
+            call()
