@@ -621,6 +621,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, freqs: tor
     rot = 2 * freqs.numel()
     if freqs.dtype is not torch.float64 or freqs.get_device() != dev or freqs.dim() != 1 or not freqs.is_contiguous() or rot > head or rot > 8192:
         raise ValueError("freqs has to be contiguous fp64 on q's device, at most half a head and 4096 long")
+    if freqs.requires_grad:
+        _frozen()
     _launch((_step_lib or _steps()).tbv_step_rotary, dev, _ROTARY.pack(
         *hq, *hk, positions.data_ptr(), freqs.data_ptr(), p0, p1, batch, tokens, head, rot, code, wide, interleaved, inverse, scale))
     if q_out is None:

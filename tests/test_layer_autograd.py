@@ -140,3 +140,23 @@ def test_outputs_that_ask_for_a_gradient_are_refused_on_gpu():
     for call in outputs_that_ask(on_gpu):
         with pytest.raises(ValueError, match="gradient"):
             call()
+
+
+def learned_frequencies(new):
+    q, k, pos, freqs = (writing_calls(new)[1][i] for i in (1, 2, 7, 8))
+    return lambda: tbvcoll.rotary(q, k, pos, freqs.requires_grad_())
+
+
+def test_frequencies_that_ask_for_a_gradient_are_refused(launches):
+    with pytest.raises(ValueError, match="gradient"):
+        learned_frequencies(stand)()
+    assert not launches
+    with torch.no_grad():
+        learned_frequencies(stand)()
+    assert len(launches) == 1
+
+
+@gpu
+def test_frequencies_that_ask_for_a_gradient_are_refused_on_gpu():
+    with pytest.raises(ValueError, match="gradient"):
+        learned_frequencies(on_gpu)()
