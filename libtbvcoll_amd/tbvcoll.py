@@ -28,6 +28,7 @@ import os
 import struct
 
 import torch
+from torch.autograd import forward_ad as _forward
 
 _DT = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _lib = None
@@ -405,6 +406,14 @@ def _frozen():
         raise ValueError("records no gradient: call it under torch.no_grad(), or in the forward and backward of a torch.autograd.Function")
 
 
+def _no_tangent(*tensors):
+    """The same for forward mode (called inside a dual level only): the kernels carry no tangent along.  In the forward of
+    a torch.autograd.Function there is none to carry, its jvp does that."""
+    for t in tensors:
+        if t is not None and _forward.unpack_dual(t).tangent is not None:
+            raise ValueError("carries no forward-mode gradient along: call it in the forward of a torch.autograd.Function that has a jvp")
+
+
 def _rows(t, shape, what):
     """(rows, columns, row stride) of a tensor of this shape as a matrix of contiguous rows; leading dimensions are taken together."""
     if len(shape) == 2:
@@ -432,6 +441,8 @@ def quantize_int8(x: torch.Tensor, codes: torch.Tensor = None, scale: torch.Tens
         raise ValueError("x has to be a fp32, fp16 or bf16 tensor on the GPU")
     if x.requires_grad:
         _frozen()
+    if _forward._current_level >= 0:
+        _no_tangent(x, scale)
     rows, cols, xs = _rows(x, shape, "x")
     given = () if codes is None and scale is None else [t for t in (codes, scale) if t is not None]
     if codes is None:
@@ -470,6 +481,8 @@ def matmul_int8(x: torch.Tensor, x_scale: torch.Tensor, w: torch.Tensor, w_scale
         raise ValueError(f"x has rows of {k} and w of {wk}: they have to be equal, and at most 131071 (beyond, the int32 sum can overflow)")
     if x_scale.requires_grad or w_scale.requires_grad or (bias is not None and bias.requires_grad):
         _frozen()
+    if _forward._current_level >= 0:
+        _no_tangent(x_scale, w_scale, bias, out)
     sx, sw = x_scale.numel(), w_scale.numel()
     if x_scale.dtype is not torch.float32 or x_scale.get_device() != dev or not x_scale.is_contiguous() or (sx != m and sx != 1):
         raise ValueError("x_scale has to be contiguous fp32 on x's device, one for each row of x or one for all")
@@ -598,6 +611,8 @@ def rotary(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, freqs: tor
         raise ValueError("q has to be fp32, fp16 or bf16 on the GPU, [tokens, heads, head] or [batch, tokens, heads, head]")
     if q.requires_grad or (k is not None and k.requires_grad):
         _frozen()
+    if _forward._current_level >= 0:
+        _no_tangent(q, k, freqs, q_out, k_out)
     batch, tokens, head = 1 if d == 3 else shape[0], shape[-3], shape[-1]
     hq = _heads(q, shape, q_out, dtype, dev, "q")
     if k is None:

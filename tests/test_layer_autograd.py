@@ -6,6 +6,7 @@ The CPU tests give the calls tensors that say they lie on a GPU and take the lau
 call does before and after it."""
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from gpu_util import say
 from libtbvcoll_amd import tbvcoll
@@ -160,3 +161,60 @@ def test_frequencies_that_ask_for_a_gradient_are_refused(launches):
 def test_frequencies_that_ask_for_a_gradient_are_refused_on_gpu():
     with pytest.raises(ValueError, match="gradient"):
         learned_frequencies(on_gpu)()
+
+
+def dual_calls(new, dual):
+    """Calls in which one tensor, read or written, carries a tangent, by its name."""
+    def d(*shape, dtype=torch.float32):
+        return dual(new(*shape, dtype=dtype))
+    x, q, k, x8, w8, s, s1, pos, freqs = writing_calls(new)[1][:9]
+    return {"x": lambda: tbvcoll.quantize_int8(d(4, 16)), "scale": lambda: tbvcoll.quantize_int8(x, scale=d(4)),
+            "x_scale": lambda: tbvcoll.matmul_int8(x8, d(4), w8, s), "w_scale": lambda: tbvcoll.matmul_int8(x8, s1, w8, d(8)),
+            "bias": lambda: tbvcoll.matmul_int8(x8, s1, w8, s, bias=d(8), dtype=torch.float32),
+            "out": lambda: tbvcoll.matmul_int8(x8, s1, w8, s, out=d(4, 8)), "q": lambda: tbvcoll.rotary(d(4, 2, 16), k, pos, freqs),
+            "a view of q": lambda: tbvcoll.rotary(d(4, 4, 16)[:, :2], None, pos, freqs),
+            "k": lambda: tbvcoll.rotary(q, d(4, 1, 16), pos, freqs), "freqs": lambda: tbvcoll.rotary(q, k, pos, d(8, dtype=torch.float64)),
+            "q_out": lambda: tbvcoll.rotary(q, k, pos, freqs, q_out=d(4, 2, 16)), "k_out": lambda: tbvcoll.rotary(q, k, pos, freqs, k_out=d(4, 1, 16))}
+
+
+def tangents_are_refused(new):
+    with forward_ad.dual_level():
+        for call in dual_calls(new, lambda t: forward_ad.make_dual(t, torch.ones_like(t))).values():
+            with torch.no_grad(), pytest.raises(ValueError, match="forward-mode"):      # (no_grad does not turn forward mode off)
+                call()
+        for call in dual_calls(new, lambda t: t).values():                              # inside a level, but none of them a dual
+            call()
+
+
+def test_tensors_with_a_tangent_are_refused(launches):
+    tangents_are_refused(stand)
+    assert len(launches) == 12
+
+
+@gpu
+def test_tensors_with_a_tangent_are_refused_on_gpu():
+    tangents_are_refused(on_gpu)
+
+
+@gpu
+@pytest.mark.parametrize("interleaved", [False, True])
+def test_rotary_jvp_in_a_function(interleaved):
+    """Forward mode as a program has it: rotation is linear, so the tangent's image is its rotation, bit for bit."""
+    pos, (freqs, _) = torch.arange(5, device="cuda") * 777, tbvcoll.rotary_frequencies(16)
+
+    def turn(v):
+        return tbvcoll.rotary(v, None, pos, freqs, interleaved=interleaved, q_out=torch.empty_like(v))[0]
+
+    class Rotary(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, q):
+            return turn(q)
+
+        @staticmethod
+        def jvp(ctx, t):
+            return turn(t)
+
+    q, t = torch.randn(5, 3, 16, device="cuda"), torch.randn(5, 3, 16, device="cuda")
+    with forward_ad.dual_level():
+        y, got = forward_ad.unpack_dual(Rotary.apply(forward_ad.make_dual(q, t)))
+    assert torch.equal(y, turn(q)) and torch.equal(got, turn(t))
