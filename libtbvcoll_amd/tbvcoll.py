@@ -523,12 +523,18 @@ def linear_int8_all_reduce(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tens
     """The row-parallel linear layer of a tensor-parallel pair with int8 weights: this rank's columns of the activations
     `x` (fp32, fp16 or bf16) as int8 rows, times this rank's columns of the weight, SUM with the peer's partial result
     (bias: on one rank only).  Returns the sum in x's type, or None when the library does not take the all-reduce (not
-    initialised, over the cap): the caller then runs its own layer."""
-    _need(x.is_cuda and x.dim() >= 1 and w.dim() == 2, "x has to be on the GPU and w a matrix")
+    initialised, over the cap): `out` is then as it was, and the caller runs its own layer.  Tensors that no call could
+    take are refused whether the library takes the all-reduce or not."""
+    dev = x.get_device()
+    _need(dev >= 0 and x.dim() >= 1 and x.dtype in _DT, "x has to be a fp32, fp16 or bf16 tensor on the GPU")
+    _need(w.dim() == 2 and w.dtype is torch.int8 and w.get_device() == dev and w.shape[1] == x.shape[-1],
+          "w has to be an int8 matrix on x's device with as many columns as x")
     n = w.shape[0]
+    _need(out is None or (out.dtype is x.dtype and out.get_device() == dev and out.shape == x.shape[:-1] + (n,) and out.is_contiguous()),
+          "out has to be contiguous, of x's type and device and of x's shape with a column for each row of w")
+    # (all that makes `all_reduce` decline is decided here, before anything is written)
     if _lib is None or math.prod(x.shape[:-1]) * n * x.element_size() > _cap:
         return None
-    _need(out is None or (out.dtype is x.dtype and out.is_contiguous()), "out has to be contiguous and of x's type")
     codes, scale = quantize_int8(x)
     out = matmul_int8(codes, scale, w, w_scale, bias=bias, out=out, dtype=x.dtype)
     return out if all_reduce(out) else None

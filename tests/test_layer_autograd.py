@@ -15,12 +15,14 @@ gpu = pytest.mark.gpu
 
 
 class Stand(torch.Tensor):
+    is_cuda = property(lambda self: True)
+
     def get_device(self):
         return 0
 
 
 def stand(*shape, dtype=torch.float32):
-    return torch.ones(*shape, dtype=dtype).as_subclass(Stand)
+    return torch.ones(shape, dtype=dtype).as_subclass(Stand)
 
 
 @pytest.fixture
@@ -32,7 +34,7 @@ def launches(monkeypatch):
 
 
 def on_gpu(*shape, dtype=torch.float32):
-    return torch.ones(*shape, dtype=dtype, device="cuda")
+    return torch.ones(shape, dtype=dtype, device="cuda")
 
 
 def writing_calls(new):

@@ -1,0 +1,51 @@
+"""Calls of the layer's operators that their documentation allows, or that they have to refuse."""
+import numpy as np
+import pytest
+import torch
+
+from gpu_util import dev, say, session
+from libtbvcoll_amd import synth, tbvcoll
+from test_layer_autograd import launches, on_gpu, stand  # noqa: F401  (a fixture)
+from test_layer_ops import DT, check, codes_of, scales_of, want_product, want_rows
+
+gpu = pytest.mark.gpu
+
+
+def bad_linear_calls(new):
+    x, w, s = new(4, 64), new(32, 64, dtype=torch.int8), new(32)
+    good = dict(x=x, w=w, w_scale=s)
+    return [good | kw for kw in (dict(x=x.double()), dict(x=new()), dict(w=w.float()), dict(w=w[:, :63]), dict(w=w.view(2, 16, 64)), dict(out=new(4, 31)),
+                                 dict(out=new(4, 32).half()), dict(out=new(32, 4).t()), dict(out=new(128)), dict(out=new(4, 64)[:, ::2]))]
+
+
+def test_row_parallel_linear_refuses_before_it_declines(launches):  # noqa: F811
+    tbvcoll.shutdown()                                                          # not initialised: every good call declines
+    x, w, s = stand(4, 64), stand(32, 64, dtype=torch.int8), stand(32)
+    assert tbvcoll.linear_int8_all_reduce(x, w, s) is None
+    for bad in bad_linear_calls(stand) + [dict(x=x, w=torch.ones(32, 64, dtype=torch.int8), w_scale=s), dict(x=x, w=w, w_scale=s, out=torch.empty(4, 32))]:
+        with pytest.raises(ValueError):
+            tbvcoll.linear_int8_all_reduce(**bad)
+    out = stand(4, 32)
+    assert tbvcoll.linear_int8_all_reduce(x, w, s, out=out) is None and bool((out == 1).all()) and not launches
+
+
+@gpu
+def test_row_parallel_linear_into_an_output():
+    x, (w, s) = dev(synth.normal(1, 4 * 64), torch.bfloat16).view(4, 64), (codes_of(1, 32, 64).cuda(), scales_of(2, 32).cuda())
+    with session(rails=1, cap=4096) as tbv:
+        one = tbv.matmul_int8(*tbv.quantize_int8(x), w, s)
+        out = torch.full((4, 32), 3.0, dtype=torch.bfloat16, device="cuda")
+        say("row-parallel linear into an output")
+        assert tbv.linear_int8_all_reduce(x, w, s, out=out) is out              # no staged peer: it echoes this rank
+        torch.cuda.synchronize()
+        assert torch.equal(out, one + one)
+        far = torch.full((132, 32), 3.0, dtype=torch.bfloat16, device="cuda")   # over the cap: declined, out as it was
+        assert tbv.linear_int8_all_reduce(x.repeat(33, 1), w, s, out=far) is None
+        torch.cuda.synchronize()
+        assert bool((far == 3.0).all())
+        none = tbv.linear_int8_all_reduce(x[:0], w, s)
+        assert none.shape == (0, 32) and none.dtype is torch.bfloat16
+        for bad in bad_linear_calls(on_gpu):
+            with pytest.raises(ValueError):
+                tbv.linear_int8_all_reduce(**bad)
+        assert not tbv.err()
