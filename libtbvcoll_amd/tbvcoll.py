@@ -535,6 +535,9 @@ def linear_int8_all_reduce(x: torch.Tensor, w: torch.Tensor, w_scale: torch.Tens
     # (all that makes `all_reduce` decline is decided here, before anything is written)
     if _lib is None or math.prod(x.shape[:-1]) * n * x.element_size() > _cap:
         return None
+    if dev != torch._C._cuda_getDevice():        # `all_reduce` takes the current device's stream: it has to be the product's
+        with torch.cuda.device(dev):
+            return linear_int8_all_reduce(x, w, w_scale, bias=bias, out=out)
     codes, scale = quantize_int8(x)
     out = matmul_int8(codes, scale, w, w_scale, bias=bias, out=out, dtype=x.dtype)
     return out if all_reduce(out) else None

@@ -1,4 +1,6 @@
 """Calls of the layer's operators that their documentation allows, or that they have to refuse."""
+import contextlib
+
 import numpy as np
 import pytest
 import torch
@@ -49,3 +51,22 @@ def test_row_parallel_linear_into_an_output():
             with pytest.raises(ValueError):
                 tbv.linear_int8_all_reduce(**bad)
         assert not tbv.err()
+
+
+def test_row_parallel_linear_runs_on_its_tensors_device(launches, monkeypatch):  # noqa: F811
+    """Tensors on another device than the current one (there is one GPU here: the devices are stand-ins)."""
+    current, seen = [1], []
+
+    @contextlib.contextmanager
+    def device(i):
+        before, current[0] = current[0], i
+        yield
+        current[0] = before
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: current[0], raising=False)
+    monkeypatch.setattr(torch.cuda, "device", device)
+    monkeypatch.setattr(tbvcoll, "_lib", tbvcoll.load())
+    monkeypatch.setattr(tbvcoll, "_cap", 1 << 20)
+    monkeypatch.setattr(tbvcoll, "all_reduce", lambda t: seen.append((current[0], list(launches))) or True)
+    assert tbvcoll.linear_int8_all_reduce(stand(4, 64), stand(32, 64, dtype=torch.int8), stand(32)).shape == (4, 32)
+    assert seen == [(0, ["tbv_step_quantize_i8", "tbv_step_matmul_i8"])] and current == [1]
