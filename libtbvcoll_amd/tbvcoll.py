@@ -415,7 +415,8 @@ def _no_tangent(*tensors):
 
 
 def _rows(t, shape, what):
-    """(rows, columns, row stride) of a tensor of this shape as a matrix of contiguous rows; leading dimensions are taken together."""
+    """(rows, columns, row stride) of a tensor of this shape as a matrix of contiguous rows; leading dimensions are taken
+    together where their rows are evenly spaced (part of the columns of a larger tensor)."""
     if len(shape) == 2:
         r, c = shape
         s, e = t.stride()
@@ -423,7 +424,15 @@ def _rows(t, shape, what):
         c, e = shape[-1], t.stride(-1)
         r, s = math.prod(shape[:-1]), c
         if len(shape) > 1 and r * c and not t.is_contiguous():
-            raise ValueError(what + ": leading dimensions have to be contiguous")
+            s, n = c, 1                          # rows are s apart: every leading dimension has to step over the ones within it
+            for size, step in zip(shape[-2::-1], t.stride()[-2::-1]):
+                if size == 1:
+                    continue
+                if n == 1:
+                    s = step
+                elif step != s * n:
+                    raise ValueError(what + ": the rows have to be evenly spaced")
+                n *= size
     else:
         raise ValueError(what + " needs at least one dimension")
     if (e != 1 and c > 1) or (s < c and r > 1):

@@ -70,3 +70,43 @@ def test_row_parallel_linear_runs_on_its_tensors_device(launches, monkeypatch): 
     monkeypatch.setattr(tbvcoll, "all_reduce", lambda t: seen.append((current[0], list(launches))) or True)
     assert tbvcoll.linear_int8_all_reduce(stand(4, 64), stand(32, 64, dtype=torch.int8), stand(32)).shape == (4, 32)
     assert seen == [(0, ["tbv_step_quantize_i8", "tbv_step_matmul_i8"])] and current == [1]
+
+
+def part(t, *leading):
+    """Columns 16 .. 79 of `leading` rows of a larger tensor."""
+    return t.view(*leading, t.shape[-1])[..., 16:80]
+
+
+def test_rows_of_part_of_a_larger_tensor():
+    t = torch.zeros(24, 112)
+    for leading in ((24,), (2, 12), (2, 3, 4), (24, 1), (1, 24), (2, 1, 12), (1, 1, 24), (2, 3, 1, 4)):
+        x = part(t, *leading)
+        assert tbvcoll._rows(x, x.shape, "x") == (24, 64, 112), leading
+    for x, want in ((part(t, 2, 12)[:, :1], (2, 64, 12 * 112)), (part(t, 2, 12)[:1, :1], (1, 64, 64)), (part(t, 2, 12)[:, ::3], (8, 64, 3 * 112)),
+                    (t.view(2, 3, 4, 112)[:, :, 0, :64], (6, 64, 448)), (t[:0].view(0, 3, 112)[..., :64], (0, 64, 64)), (t.view(2, 12, 112)[..., 5:6], (24, 1, 112))):
+        assert tbvcoll._rows(x, x.shape, "x") == want
+    for x in (part(t, 2, 12)[:, :5], t.view(2, 12, 112).transpose(0, 1), t.view(2, 12, 112).transpose(1, 2), t[:, None].expand(24, 2, 112),
+              part(t, 2, 12).expand(3, 2, 12, 64), t.view(2, 3, 4, 112)[:, :, :2], t[None, :1].expand(5, 1, 112)):
+        with pytest.raises(ValueError):
+            tbvcoll._rows(x, x.shape, "x")
+
+
+@gpu
+@pytest.mark.parametrize("name", list(DT))
+@pytest.mark.parametrize("leading", [(2, 12), (2, 3, 4), (24, 1), (1, 24)])
+def test_batches_that_are_part_of_a_larger_tensor(name, leading):
+    """The columns of a packed projection, [batch, tokens, part of the columns]: read, and written with the rest left as it was."""
+    dt = DT[name]
+    x = part(dev(synth.normal(1, 24 * 112), dt).view(24, 112), *leading)
+    store = torch.full((24, 112), 77, dtype=torch.int8, device="cuda")
+    say("part of a larger tensor", name, leading)
+    codes, scale = tbvcoll.quantize_int8(x, codes=part(store, *leading))
+    c, s = want_rows(x)
+    assert torch.equal(codes.cpu(), c) and torch.equal(scale.cpu(), s)
+    assert torch.equal(tbvcoll.quantize_int8(x)[0], codes)
+    w, ws = codes_of(2, 64, 64).cuda(), scales_of(3, 64).cuda()
+    wide = torch.full((24, 112), 5.0, dtype=dt, device="cuda")
+    tbvcoll.matmul_int8(codes, scale, w, ws, out=part(wide, *leading))
+    want, before = want_product(c.reshape(24, 64), s.reshape(24), w, ws, None)
+    check(wide[:, 16:80], want, before, dt, (name, leading))
+    assert all(bool((t[:, :16] == v).all() and (t[:, 80:] == v).all()) for t, v in ((store, 77), (wide, 5.0)))
