@@ -6,7 +6,8 @@
 // of the first `rot` elements of a head; the rest is copied.  The inverse is the transpose of the rotation, so it is
 // the backward pass of a forward call with the same `scale`.  The angle is formed and reduced to a fraction of a turn
 // in fp64 (positions of a million lose 16 of fp32's 24 bits to whole turns); everything after it is fp32, the result
-// is rounded once to the storage type.
+// is rounded once to the storage type.  The steps are written out (`turned`, `fp32_value`), so that an element's bits do not
+// depend on which variant of the kernel computes it: in place or not, alone or among many tokens.
 // No counterpart in the reference: it is what lies between the product that follows its all-reduce and the attention.
 #include <hip/hip_runtime.h>
 #include <stdio.h>
@@ -38,6 +39,22 @@ struct RotArgs {
     bool through;                               // write them through the L2
 };
 
+// A pair turned: one rounded product, then one fused multiply-add.
+__device__ __forceinline__ float2 turned(float x1, float x2, float2 w)
+{
+    return make_float2(__builtin_fmaf(x1, w.x, -(x2 * w.y)), __builtin_fmaf(x2, w.x, x1 * w.y));
+}
+
+// The value in fp32, whatever it becomes next.  Left to itself the compiler merges some of the multiply-adds with the rounding to
+// fp16 that follows (one rounding in place of two, so some results differ), others not, from variant to variant.
+__device__ __forceinline__ float fp32_value(float v)
+{
+#ifdef __HIP_DEVICE_COMPILE__          // (a register constraint the host pass does not know)
+    asm("" : "+v"(v));
+#endif
+    return v;
+}
+
 template <int DT> __device__ __forceinline__ float rot_load(const void* p, ptrdiff_t i)
 {
     if (DT == 0) return ((const float*)p)[i];
@@ -47,7 +64,7 @@ template <int DT> __device__ __forceinline__ float rot_load(const void* p, ptrdi
 template <int DT> __device__ __forceinline__ void rot_store(void* p, ptrdiff_t i, float v)
 {
     if (DT == 0) ((float*)p)[i] = v;
-    else if (DT == 1) ((_Float16*)p)[i] = (_Float16)v;
+    else if (DT == 1) ((_Float16*)p)[i] = (_Float16)fp32_value(v);
     else ((__bf16*)p)[i] = (__bf16)v;
 }
 template <int DT> __device__ __forceinline__ void rot_copy(void* o, ptrdiff_t j, const void* p, ptrdiff_t i)
@@ -108,7 +125,7 @@ template <int DT> struct Lanes {                      // 16 bytes as fp32 and ba
         typedef T T8 __attribute__((ext_vector_type(8)));
         T8 o;
 #pragma unroll
-        for (int i = 0; i < 8; i++) o[i] = (T)f[i];
+        for (int i = 0; i < 8; i++) o[i] = (T)(DT == 1 ? fp32_value(f[i]) : f[i]);
         return __builtin_bit_cast(u32x4, o);
     }
 };
@@ -198,16 +215,16 @@ __global__ __launch_bounds__(512) void k_rotary(RotArgs g, unsigned total)
                     if (INTER) {
 #pragma unroll
                         for (unsigned e = 0; e < P; e++) {
-                            p[2 * e] = x[2 * e] * w[e].x - x[2 * e + 1] * w[e].y;
-                            p[2 * e + 1] = x[2 * e + 1] * w[e].x + x[2 * e] * w[e].y;
+                            const float2 v = turned(x[2 * e], x[2 * e + 1], w[e]);
+                            p[2 * e] = v.x; p[2 * e + 1] = v.y;
                         }
                         store16<THROUGH>(g.base, out[u] + i * 16, Lanes<DT>::pack(p));
                     } else {
                         Lanes<DT>::unpack(b[u], y);
 #pragma unroll
                         for (unsigned e = 0; e < P; e++) {
-                            p[e] = x[e] * w[e].x - y[e] * w[e].y;
-                            q[e] = y[e] * w[e].x + x[e] * w[e].y;
+                            const float2 v = turned(x[e], y[e], w[e]);
+                            p[e] = v.x; q[e] = v.y;
                         }
                         store16<THROUGH>(g.base, out[u] + i * 16, Lanes<DT>::pack(p));
                         store16<THROUGH>(g.base, out[u] + i * 16 + apart, Lanes<DT>::pack(q));
@@ -222,8 +239,9 @@ __global__ __launch_bounds__(512) void k_rotary(RotArgs g, unsigned total)
 #pragma unroll
                 for (int u = 0; u < U; u++) {
                     if (u >= live) break;
-                    rot_store<DT>(out[u], j1, x1[u] * w.x - x2[u] * w.y);
-                    rot_store<DT>(out[u], j2, x2[u] * w.x + x1[u] * w.y);
+                    const float2 v = turned(x1[u], x2[u], w);
+                    rot_store<DT>(out[u], j1, v.x);
+                    rot_store<DT>(out[u], j2, v.y);
                 }
             } else {
 #pragma unroll
