@@ -1,10 +1,13 @@
 """Calls of the layer's operators that their documentation allows, or that they have to refuse."""
 import contextlib
+import os
+import subprocess
+import sys
 
-import numpy as np
 import pytest
 import torch
 
+import test_layer_ops
 from gpu_util import dev, say, session
 from libtbvcoll_amd import synth, tbvcoll
 from test_layer_autograd import launches, on_gpu, stand  # noqa: F401  (a fixture)
@@ -110,3 +113,16 @@ def test_batches_that_are_part_of_a_larger_tensor(name, leading):
     want, before = want_product(c.reshape(24, 64), s.reshape(24), w, ws, None)
     check(wide[:, 16:80], want, before, dt, (name, leading))
     assert all(bool((t[:, :16] == v).all() and (t[:, 80:] == v).all()) for t, v in ((store, 77), (wide, 5.0)))
+
+
+@gpu
+@pytest.mark.parametrize("work", ["graph_and_two_streams()", "two_threads()", "autograd_function(False)", "autograd_function(True)", "FIRST_CALL_IN_A_CAPTURE"])
+def test_a_process_with_graphs_and_streams_ends_well(work):
+    """The work that the other tests run in processes of its own: here the process has to end with status 0 as well, its
+    graphs and streams taken down."""
+    say(work, "in a process of its own")
+    code = f"import sys; sys.path[:0] = [{test_layer_ops.ROOT!r}, {os.path.join(test_layer_ops.ROOT, 'tests')!r}]; import test_layer_ops as t; t.{work}; print('DONE', flush=True)"
+    if work == "FIRST_CALL_IN_A_CAPTURE":
+        code = test_layer_ops.FIRST_CALL_IN_A_CAPTURE.format(root=test_layer_ops.ROOT) + "print('DONE', flush=True)\n"
+    p = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=110)
+    assert p.returncode == 0 and "DONE" in p.stdout and "False" not in p.stdout, (p.returncode, p.stdout[-1000:], p.stderr[-3000:])
