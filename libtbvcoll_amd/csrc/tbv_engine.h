@@ -140,6 +140,7 @@ struct Engine {
     int wire_mode = 0;                        // TBV_WIRE: 0 auto (probe each new caller stream), 1 stream, 2 host
     void* wire_stream = nullptr;              // the caller stream of the verdict below (the usual case: one stream)
     bool wire_stream_host = false;
+    bool wire_stream_known = false;           // there is such a verdict (a null wire_stream is a caller's default stream)
     std::vector<std::pair<void*, bool>> stream_wire;   // every probed caller stream -> use the host wire
     // a pack's completion word that its kernel did not raise: the next kernel on the same stream raises it
     PreSignal pending;

@@ -317,14 +317,14 @@ bool use_host_wire(hipStream_t st)
 {
     if (G.wire_mode == 2) return true;
     if (G.wire_mode == 1) return false;
-    if ((void*)st == G.wire_stream) return G.wire_stream_host;        // the usual case: the stream of the call before
+    if (G.wire_stream_known && (void*)st == G.wire_stream) return G.wire_stream_host;        // the usual case: the stream of the call before
     bool host = false, known = false;
     for (auto& p : G.stream_wire) if (p.first == (void*)st) { host = p.second; known = true; break; }
     if (!known) {
         host = shares_queue_with_wire(st) && dma_ready();
         G.stream_wire.emplace_back((void*)st, host);
     }
-    G.wire_stream = (void*)st; G.wire_stream_host = host;
+    G.wire_stream = (void*)st; G.wire_stream_host = host; G.wire_stream_known = true;
     return host;
 }
 
@@ -373,7 +373,7 @@ void peer_teardown()
     G.owned.clear();
     if (G.resident_src) { (void)hipFree(G.resident_src); G.resident_src = nullptr; }
     G.resident_bytes = 0;
-    G.stream_wire.clear(); G.wire_stream = nullptr; G.wire_stream_host = false;
+    G.stream_wire.clear(); G.wire_stream = nullptr; G.wire_stream_host = G.wire_stream_known = false;
     G.staged.clear(); G.repeat = Staged{nullptr, 0, false};
     G.script.clear(); G.turn.store(0); G.withhold_seq.store(0); G.hooks = 0;
     for (int r = 0; r < MAXRAIL; r++) G.hold[r].store(0);
