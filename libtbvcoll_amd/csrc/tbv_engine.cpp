@@ -356,6 +356,7 @@ int configure(const char* devs, size_t cap)
     G.fusewait_max = getz("TBV_FUSEWAIT", (size_t)1 << 20);
     G.defer = geti("TBV_DEFERSIG", 1);
     G.onekernel = geti("TBV_ONEKERNEL", 1);
+    { const char* e = getenv("TBV_PROBEDELAY"); G.probe_delay_us = e ? std::min(1e6, std::max(0.0, atof(e))) : 0.0; }
     { const char* e = getenv("TBV_WIRE");
       G.wire_mode = (e && !strcmp(e, "stream")) ? 1 : (e && !strcmp(e, "host")) ? 2 : 0; }
     G.stride = G.cap + (G.tag ? 4096 : 0);

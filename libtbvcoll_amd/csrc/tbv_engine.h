@@ -137,6 +137,7 @@ struct Engine {
     std::vector<std::pair<uint64_t, int>> arrivals;
     std::atomic<int> probe{0};
     std::vector<double> latencies;
+    double probe_delay_us = 0;                // test hook: the host is held up this long in the middle of a probe (TBV_PROBEDELAY)
     int wire_mode = 0;                        // TBV_WIRE: 0 auto (probe each new caller stream), 1 stream, 2 host
     void* wire_stream = nullptr;              // the caller stream of the verdict below (the usual case: one stream)
     bool wire_stream_host = false;
@@ -178,6 +179,7 @@ inline unsigned long long* rflag(int rail, int s) { return word(W_RFLAG0 + rail,
 inline unsigned long long* footprints() { return word(W_MISC, 0); }     // 8 words
 inline unsigned long long* dbgwords() { return word(W_MISC, 2); }       // 8 words
 inline unsigned long long* scratchword() { return word(W_MISC, 4); }
+inline unsigned long long* probewords() { return word(W_MISC, 5); }     // 8 words
 
 inline uint64_t ld_acq(const unsigned long long* p) { return __atomic_load_n(p, __ATOMIC_ACQUIRE); }
 inline void st_rel(unsigned long long* p, uint64_t v) { __atomic_store_n(p, (unsigned long long)v, __ATOMIC_RELEASE); }

@@ -65,23 +65,33 @@ int host_deposit(Rail& x, const Item& it, size_t off, size_t len, double t0)
 // multiplexes streams onto a few hardware queues; two streams on one queue run in submission order,
 // so a side-stream copy submitted after the caller's gate would sit behind the gate it is meant to
 // release.  Probe: a wait kernel bounded to 300 us goes on the caller's stream, the word it waits
-// for is raised from the side stream; on separate queues the wait ends at once, on a shared queue it
-// runs to its bound.  Every kernel involved exits by itself.
+// for is raised from the side stream; on separate queues the wait ends with the word, on a shared queue
+// it runs to its bound.  Which of the two is what the kernel itself says (a host clock does not: a thread that
+// is held up between the launch and its first look at the clock sees a short wait either way).  A host that is slow to
+// raise the word makes separate queues look shared, so that answer is asked for three times; the other way round
+// no delay can.  Every kernel involved exits by itself.
 bool shares_queue_with_wire(hipStream_t st)
 {
     if (hipStreamSynchronize(st) != hipSuccess) { (void)hipGetLastError(); return true; }   // measure queues, not backlog
     for (int r = 0; r < G.R; r++) {
-        unsigned long long* w = scratchword();
-        st_rel(w, 0);
-        if (launch_waitflag(w, 1, (unsigned long long)(300e-6 * G.tick_hz), nullptr, st) != hipSuccess) return true;
-        const double t0 = nowt();
-        if (stream_bump(G.rr[r].wire, w, 1) != hipSuccess) { (void)hipStreamSynchronize(st); return true; }
-        while (hipStreamQuery(st) == hipErrorNotReady && nowt() - t0 < 0.05) { }
-        const double dt = nowt() - t0;
-        (void)hipStreamSynchronize(G.rr[r].wire);
-        (void)hipStreamSynchronize(st);
-        (void)hipGetLastError();
-        if (dt > 200e-6) {
+        unsigned long long *w = scratchword(), *fp = probewords();
+        bool apart = false;
+        double dt = 0;
+        for (int attempt = 0; attempt < 3 && !apart; attempt++) {
+            st_rel(w, 0);
+            st_rel(fp + FP_WAIT_TIMEOUT, 0);
+            const double t0 = nowt();
+            if (launch_waitflag(w, 1, (unsigned long long)(300e-6 * G.tick_hz), fp, st) != hipSuccess) return true;
+            if (G.probe_delay_us > 0) for (const double ts = nowt(); nowt() - ts < G.probe_delay_us * 1e-6; ) { }
+            if (stream_bump(G.rr[r].wire, w, 1) != hipSuccess) { (void)hipStreamSynchronize(st); return true; }
+            while (hipStreamQuery(st) == hipErrorNotReady && nowt() - t0 < 0.05) { }
+            dt = nowt() - t0;
+            (void)hipStreamSynchronize(G.rr[r].wire);
+            (void)hipStreamSynchronize(st);
+            (void)hipGetLastError();
+            apart = ld_acq(fp + FP_WAIT_TIMEOUT) == 0;
+        }
+        if (!apart) {
             LOGF("stream %p shares a hardware queue with rail%d's side stream (probe %.0f us): using the host wire for it",
                  (void*)st, r, dt * 1e6);
             return true;

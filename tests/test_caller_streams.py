@@ -43,3 +43,14 @@ def test_the_default_stream_with_many_streams_alive():
         with session(rails=2, cap=1 << 20, TBV_WDOG=5) as tbv:
             say("default stream beside", len(streams), "others")
             exact_calls(tbv, 50 + i)
+
+
+def test_a_host_that_is_held_up_during_the_probe(capfd):
+    """The wait is over by its bound before the host looks: that says nothing of separate queues, so the calls take the way
+    that works on either."""
+    with session(rails=2, cap=1 << 20, TBV_WDOG=5, TBV_PROBEDELAY=1000) as tbv:
+        capfd.readouterr()
+        say("probe with the host held up")
+        exact_calls(tbv, 70)
+        err = capfd.readouterr().err
+        assert "shares a hardware queue" in err and "separate hardware queues" not in err, err
