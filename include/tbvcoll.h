@@ -149,7 +149,7 @@ int tbv_step_noalloc(void* out, const void* local, const void* received, void* b
  * no counterpart in the reference.  Like tbv_step_noalloc they work on the caller's buffers only: no tbv_ar_init, no
  * allocation, no workspace, no state between calls; any thread, any stream, stream capture included (the device of
  * `stream` must be current).  Return 0; -1 after a "[tbvcoll] ..." line on stderr for bad arguments or a launch failure.
- * Strides are in elements; the last dimension is contiguous. */
+ * Strides are in elements, up to 2^30 (rotary: 2^56 for a whole dimension); the last dimension is contiguous. */
 
 /* Rows of `hidden` elements of `dtype` to int8 codes and one fp32 scale a row:
  *   scale = max(f32(max|x| / 127), 2^-126),  code = x / scale to the nearest integer, ties to even (decided exactly).
@@ -167,7 +167,7 @@ int tbv_step_quantize_i8(const tbv_quantize_i8* call, void* stream);
 /* out[m, n] = T(float(sum over k of x[m, k] * w[n, k]) * x_scale[m] * w_scale[n] + bias[n])
  * x: m rows of k int8, w: n rows of k int8 (a linear layer's weight as stored); the sum is exact in int32 (hence the
  * largest k), the rest fp32, rounded once to `dtype`.  x_scales is m or 1 (one scale for all rows), w_scales n or 1;
- * bias (n elements of `dtype`) may be NULL.  k = 0 gives the bias.  out must not overlap an operand.
+ * bias (n elements of `dtype`) may be NULL.  k = 0: every sum is 0.  out must not overlap an operand.
  * Fast when x and w are 16-byte aligned and k and their strides multiples of 16; any other layout works. */
 #define TBV_MATMUL_I8_MAX_K 131071
 typedef struct {

@@ -87,9 +87,9 @@ __global__ __launch_bounds__(256) void k_mat_short(MatArgs g)
 // the last fragment of t has been read.  Fragments are read half a step ahead of the products that use them, so a step has
 // one barrier and no product waits for the LDS; two blocks share a CU where 80 KB of LDS do for one.  G groups of four waves take the steps in turn and join their sums in the LDS,
 // for products with fewer tiles than the GPU has CUs.
-// What bounds it (2048 x 8192 x 4096 bf16 61 us, 8192 x 8192 x 4096 217-232 us: 2.24 and 2.4-2.5 POP/s, the library's product alone
-// takes 68 and 245): the matrix units, busy 68 % of the cycles, at the clock that the power limit leaves (1.85 GHz; the same
-// product of zeros takes three quarters of the time).
+// What bounds it (2048 x 8192 x 4096 bf16 60-62 us, 8192 x 8192 x 4096 217-232 us: 2.2-2.3 and 2.4-2.5 POP/s, the library's product
+// alone takes 68 and 245): the matrix units, busy 66 and 71 % of the cycles, at the clock that the power limit leaves (1.85 GHz; the
+// same product of zeros takes three quarters of the time).  What the units wait for in the other cycles is not measured.
 typedef __attribute__((address_space(3))) void lds_void;
 
 template <int N> struct Int { static constexpr int value = N; };
@@ -646,7 +646,8 @@ template <int DT> void launch_mat(const MatArgs& g, hipStream_t st)
         case 9: return launch_tile<DT, 2, 4, 3, 1>(g, st);
         default: break;
     }
-    // A result that the caches do not hold until it is read is stored past them, others are written through the L2.  Ordinary
+    // A result of this tile that the caches do not hold until it is read is stored past them, others are written through the L2, as
+    // the other tiles' results are at any size (few as large as this take one of those; not measured there).  Ordinary
     // stores, through, past, alone and with a copy of the result behind the product, in us: 17 MB (2048 x 4096 bf16, k = 4096) 36.8,
     // 36.1, 36.6 and 42.8, 42.1, 44.1; 34 MB (2048 x 8192) 60.8, 59.1, 59.6 and 70.6, 68.7, 72.7; 134 MB (8192 x 8192) 233, 232, 227
     // and 287, 285, 282.

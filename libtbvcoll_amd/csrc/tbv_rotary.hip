@@ -266,7 +266,8 @@ template <int DT> void launch_rot(const RotArgs& g, bool inter, unsigned total, 
     // copied (two: 22.2 instead of 20.0 us for 8191 tokens of 20 heads of 128 fp16, 64 of them turned in interleaved pairs;
     // 31.0 instead of 27.4 for 4096 tokens of 40 heads of 96, 46 turned), otherwise two (one: 12.6 instead of 11.3 us for 2048
     // tokens of 40 heads of 128 bf16, 24.7 instead of 20.1 for 4096 interleaved), but one in the half layout beyond
-    // 4096 tokens (two: 36.4 instead of 34.0 us for 8192).
+    // 4096 tokens (two: 36.4 instead of 34.0 us for 8192).  Below 1024 tokens, four blocks for each CU, more heads to a thread leave
+    // CUs without work.  The step at 4096 was fitted at 40 heads of 128 and is in tokens: other heads move other bytes by then.
     const unsigned per = total < 1024 || heads == 1 ? 1 : copies ? 4 : inter || total <= 4096 ? 2 : 1;
     const unsigned want = (heads + per - 1) / per, y = want < 512 / x ? want : 512 / x;
     // small heads of many tokens: more than one token to a block, as long as the GPU is filled
