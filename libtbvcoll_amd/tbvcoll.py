@@ -453,7 +453,7 @@ def quantize_int8(x: torch.Tensor, codes: torch.Tensor = None, scale: torch.Tens
     if _forward._current_level >= 0:
         _no_tangent(x, scale)
     rows, cols, xs = _rows(x, shape, "x")
-    given = () if codes is None and scale is None else [t for t in (codes, scale) if t is not None]
+    given = () if codes is None else (codes,)
     if codes is None:
         codes = torch.empty_like(x, dtype=torch.int8) if x.is_contiguous() else x.new_empty(shape, dtype=torch.int8)
         cs = cols
@@ -463,10 +463,12 @@ def quantize_int8(x: torch.Tensor, codes: torch.Tensor = None, scale: torch.Tens
         cs = _rows(codes, shape, "codes")[2]
     if scale is None:
         scale = x.new_empty(shape[:-1], dtype=torch.float32)
-    elif scale.dtype is not torch.float32 or scale.shape != shape[:-1] or scale.get_device() != dev or not scale.is_contiguous():
-        raise ValueError("scale has to be contiguous fp32, of x's shape without its last dimension, on its device")
-    elif scale.requires_grad:
-        _frozen()
+    else:
+        if scale.dtype is not torch.float32 or scale.shape != shape[:-1] or scale.get_device() != dev or not scale.is_contiguous():
+            raise ValueError("scale has to be contiguous fp32, of x's shape without its last dimension, on its device")
+        if scale.requires_grad:
+            _frozen()
+        given += (scale,)
     if rows:
         _launch((_step_lib or _steps()).tbv_step_quantize_i8, dev, _QUANTIZE.pack(codes.data_ptr(), scale.data_ptr(), x.data_ptr(), cs, xs, rows, cols, code))
         if given:

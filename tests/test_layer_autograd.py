@@ -220,3 +220,14 @@ def test_rotary_jvp_in_a_function(interleaved):
     with forward_ad.dual_level():
         y, got = forward_ad.unpack_dual(Rotary.apply(forward_ad.make_dual(q, t)))
     assert torch.equal(y, turn(q)) and torch.equal(got, turn(t))
+
+
+def test_a_leaf_written_under_no_grad_moves_on(launches):
+    with torch.no_grad():
+        for call, leaf in ((lambda t: tbvcoll.quantize_int8(stand(4, 16), scale=t), stand(4)),
+                           (lambda t: tbvcoll.matmul_int8(stand(4, 16, dtype=torch.int8), stand(1), stand(8, 16, dtype=torch.int8), stand(1), out=t), stand(4, 8))):
+            leaf.requires_grad_()
+            before = leaf._version
+            call(leaf)
+            assert leaf._version > before
+    assert len(launches) == 2
