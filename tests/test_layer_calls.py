@@ -3,13 +3,14 @@ import contextlib
 import os
 import subprocess
 import sys
+from types import SimpleNamespace
 
 import pytest
 import torch
 
 import test_layer_ops
 from gpu_util import dev, say, session
-from libtbvcoll_amd import synth, tbvcoll
+from libtbvcoll_amd import synth, tbvcoll, vllm_intercept
 from test_layer_autograd import launches, on_gpu, stand  # noqa: F401  (a fixture)
 from test_layer_ops import DT, check, codes_of, scales_of, want_product, want_rows
 
@@ -126,3 +127,30 @@ def test_a_process_with_graphs_and_streams_ends_well(work):
         code = test_layer_ops.FIRST_CALL_IN_A_CAPTURE.format(root=test_layer_ops.ROOT) + "print('DONE', flush=True)\n"
     p = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=110)
     assert p.returncode == 0 and "DONE" in p.stdout and "False" not in p.stdout, (p.returncode, p.stdout[-1000:], p.stderr[-3000:])
+
+
+@gpu
+def test_an_empty_batch_through_the_intercept():
+    """No tokens (null pointers): nothing to sum, and the calls after it find the ring as it was."""
+    class Group:
+        unique_name, world_size = "tp:0", 2
+
+        def all_reduce(self, t):
+            return t * 3
+
+    ps = SimpleNamespace(GroupCoordinator=Group, get_tp_group=Group)
+    x, (w, s) = dev(synth.normal(1, 4 * 64), torch.bfloat16).view(4, 64), (codes_of(1, 32, 64).cuda(), scales_of(2, 32).cuda())
+    tbvcoll.shutdown()
+    one = tbvcoll.matmul_int8(*tbvcoll.quantize_int8(x), w, s)
+    ic = vllm_intercept.install(ps, 0, "rail0", cap_bytes=4096)
+    try:
+        for i in range(10):                                                      # more calls than the ring has slots
+            say("empty batch", i)
+            none = ic.row_linear_int8(Group(), x[:0], w, s)
+            assert none.shape == (0, 32) and none.dtype is torch.bfloat16
+            assert torch.equal(ic.row_linear_int8(Group(), x, w, s), one + one)  # through the library (echoing peer)
+        torch.cuda.synchronize()
+        assert not tbvcoll.err()
+    finally:
+        ic.uninstall()
+        tbvcoll.shutdown()
