@@ -3,7 +3,8 @@
 //   out[m, n] = T(float(sum_k x[m, k] * w[n, k]) * x_scale[m] * w_scale[n] + bias[n])
 //
 // The sum is exact in int32 (k <= 131071), so neither the split nor the order of a tile's work shows in the result;
-// conversion, the two products and the bias are fp32, the result is rounded once to T.
+// conversion, the two products and the bias are fp32, the result is rounded once to T (fp16: the last multiply-add straight to fp16,
+// in every kernel alike; a test holds a row's bits over all of them).
 // No counterpart in the reference: it is the product whose output its all-reduce sums.
 #include <hip/hip_runtime.h>
 #include <stdio.h>
